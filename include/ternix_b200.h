@@ -261,6 +261,34 @@ int ternix_b200_matmul_dequant(const int8_t *dA, const uint8_t *dW, void *const 
                                const float *d_row_scale, float w_scale, int M, int K, int N, long long ldy,
                                int32_t *d_status, void *stream);
 
+/* ---- a quantised layer around the product ----------------------------------------------------------------------
+ * The reference has the float halves of these steps as host functions that nothing calls (RMSNorm and SwiGLU,
+ * src/simd_math.cpp:7-46) and no activation scaling; here they are fused with the quantiser that the product needs.
+ * All arithmetic is fp32, stated so that it can be checked:
+ *   rmsnorm_quantize: h = T(x + residual), written to dH (without a residual h = x and dH is NULL);
+ *                     t = f32(h * weight) (weight NULL: t = h);  s = 1 / sqrt(mean_k h^2 + eps);
+ *   glu_quantize:     z = act(gate) * up;  with norm: t = f32(z * weight), s = 1 / sqrt(mean_k z^2 + eps);  else t = z, s = 1;
+ *   both:             m = max_k |t|;  q = rint(t * (127 / m)), ties to even;  row_scale = (m / 127) * s.
+ * A row of zeros gets codes 0 and row_scale 1.  A row with an infinity or a NaN in t, or whose sum of squares leaves
+ * fp32, gets codes 0 and row_scale NaN: what is computed from it is NaN, as it is without quantisation.
+ * x, residual, h, gate and up have type *_dtype and row pitches in elements (columns are contiguous; any alignment of an
+ * element); weight has the same type or float32.  dA is [M,K] without gaps, as the product takes it.  dH may be dX or
+ * dResidual itself (not a shifted view of them); no other output may overlap an input.  eps in [1e-12, 1].
+ * Asynchronous on `stream`; no workspace. */
+#define TERNIX_B200_DTYPE_F16   2   /* here and in ternix_b200_matmul_fused */
+#define TERNIX_B200_ACT_NONE       0
+#define TERNIX_B200_ACT_RELU       1
+#define TERNIX_B200_ACT_RELU2      2   /* max(v, 0)^2 */
+#define TERNIX_B200_ACT_SILU       3   /* v / (1 + exp(-v)) */
+#define TERNIX_B200_ACT_GELU       4   /* v (1 + erf(v / sqrt 2)) / 2 */
+#define TERNIX_B200_ACT_GELU_TANH  5   /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+int ternix_b200_rmsnorm_quantize(const void *dX, long long ldx, const void *dResidual, long long ldr, int x_dtype,
+                                 const void *dWeight, int w_dtype, float eps, void *dH, long long ldh, int8_t *dA,
+                                 float *d_row_scale, int M, int K, void *stream);
+int ternix_b200_glu_quantize(const void *dGate, long long ldg, const void *dUp, long long ldu, int dtype, int activation,
+                             int norm, const void *dWeight, int w_dtype, float eps, int8_t *dA, float *d_row_scale, int M,
+                             int K, void *stream);
+
 /* ---- N-column sharding plan (host arithmetic only) ---------------------------------------------
  * Splits N columns over `world` ranks in granules of `granule` columns (a multiple of 4; 64 keeps each
  * shard's packed rows 16-byte aligned).  Writes the first column and the column count of `rank`.

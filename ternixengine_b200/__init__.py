@@ -55,6 +55,7 @@ EXPORTS = (
     "ternix_b200_prepack_k4", "ternix_b200_prepack_k4_bytes", "ternix_b200_group_run", "ternix_b200_group_launches", "ternix_b200_group_destroy",
     "ternix_b200_gemv_batch_noalloc", "ternix_b200_gemv_batch_noalloc_limits",
     "ternix_b200_quantize_rows", "ternix_b200_matmul_dequant",
+    "ternix_b200_rmsnorm_quantize", "ternix_b200_glu_quantize",
     "ternix_b200_matmul_bcast", "ternix_b200_peer_alloc", "ternix_b200_peer_free", "ternix_b200_peer_export",
     "ternix_b200_peer_import", "ternix_b200_peer_close", "ternix_b200_peer_barrier",
     "ternix_b200_shard_columns", "ternix_b200_unpack_gathered",
@@ -117,6 +118,8 @@ def _load() -> ctypes.CDLL:
         "ternix_b200_gemv_batch_noalloc": (i32, [c.POINTER(_Problem), i32, vp, vp]),
         "ternix_b200_gemv_batch_noalloc_limits": (i32, [c.POINTER(i32), c.POINTER(i32), c.POINTER(i64)]),
         "ternix_b200_quantize_rows": (i32, [vp, i32, i64, vp, vp, i32, i32, vp]),
+        "ternix_b200_rmsnorm_quantize": (i32, [vp, i64, vp, i64, i32, vp, i32, c.c_float, vp, i64, vp, vp, i32, i32, vp]),
+        "ternix_b200_glu_quantize": (i32, [vp, i64, vp, i64, i32, i32, i32, vp, i32, c.c_float, vp, vp, i32, i32, vp]),
         "ternix_b200_matmul_dequant": (i32, [vp, vp, c.POINTER(vp), i32, vp, c.c_float, i32, i32, i32, i64, vp, vp]),
         "ternix_b200_matmul_bcast": (i32, [vp, vp, c.POINTER(vp), i32, i32, i32, i32, i64, vp, vp]),
         "ternix_b200_peer_alloc": (i32, [c.POINTER(vp), sz]),
@@ -403,6 +406,135 @@ def matmul_dequant(a, w_packed, row_scale, w_scale: float, out=None, status=None
                                               status.data_ptr() if status is not None else None,
                                               torch.cuda.current_stream(a.device).cuda_stream), "matmul_dequant")
     return out
+
+
+# --------------------------------------------------------------------------- a quantised layer around the product
+ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
+
+
+def _dtype_codes():
+    import torch
+
+    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _OnDevice:
+    """Makes a device current for a library call where it is not already, and hands out the address of the current
+    stream of that device."""
+
+    __slots__ = ("_guard", "_device")
+
+    def __init__(self, device):
+        import torch
+
+        self._device = device
+        self._guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        import torch
+
+        if self._guard is not None:
+            self._guard.__enter__()
+        return torch.cuda.current_stream(self._device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _rows(t, name, device, dtype, shape):
+    """Checks a row-major operand with unit column stride and returns (address, row pitch in elements)."""
+    M, K = shape
+    if t.device != device or t.dtype != dtype or tuple(t.shape) != shape or (K > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be {shape} {dtype} on {device} with unit column stride")
+    ld = t.stride(0) if M > 1 else K
+    if ld < K:
+        raise ValueError(f"{name}: its rows overlap")
+    return t.data_ptr(), ld
+
+
+def _flat(t, name, device, dtypes, n):
+    if t.device != device or t.dtype not in dtypes or tuple(t.shape) != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be ({n},) of {' or '.join(str(d) for d in dtypes)} on {device}, contiguous")
+    return t.data_ptr()
+
+
+def _quantized_out(x, out, row_scale):
+    import torch
+
+    M, K = x.shape
+    if out is None:
+        out = torch.empty((M, K), dtype=torch.int8, device=x.device)
+    elif out.device != x.device or out.dtype != torch.int8 or tuple(out.shape) != (M, K) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous ({M}, {K}) int8 tensor on {x.device}")
+    if row_scale is None:
+        row_scale = torch.empty((M,), dtype=torch.float32, device=x.device)
+    _flat(row_scale, "row_scale", x.device, (torch.float32,), M)
+    return out, row_scale
+
+
+def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None, row_scale=None, residual_out=None):
+    """The step in front of a quantised projection: h = x + residual (rounded to x's type), y = h / rms(h) * weight, and
+    y as int8 codes with one float32 scale per row, in one pass on the current stream (ternix_b200_rmsnorm_quantize).
+
+    x, residual: CUDA (M, K) bfloat16, float16 or float32, unit column stride, any row pitch.  weight: (K,) of the same
+    type or float32, or None.  Returns (codes, row_scale), and h as a third where a residual is given; residual_out may be
+    `residual` or `x` itself.  codes x row_scale stands for y: codes = rint(h * weight * 127 / max|h * weight|).  A row of
+    zeros has codes 0 and scale 1, a row with an infinity or NaN has codes 0 and scale NaN."""
+    import torch
+
+    codes = _dtype_codes()
+    if not x.is_cuda or x.dim() != 2 or x.dtype not in codes:
+        raise ValueError("rmsnorm_quantize takes a CUDA (M, K) bfloat16, float16 or float32 tensor")
+    M, K = x.shape
+    px, ldx = _rows(x, "x", x.device, x.dtype, (M, K))
+    pr = ph = pw = None
+    ldr = ldh = w_dtype = 0
+    if weight is not None:
+        pw, w_dtype = _flat(weight, "weight", x.device, (x.dtype, torch.float32), K), codes.get(weight.dtype)
+    out, row_scale = _quantized_out(x, out, row_scale)
+    if residual is not None:
+        pr, ldr = _rows(residual, "residual", x.device, x.dtype, (M, K))
+        if residual_out is None:
+            residual_out = torch.empty((M, K), dtype=x.dtype, device=x.device)
+        ph, ldh = _rows(residual_out, "residual_out", x.device, x.dtype, (M, K))
+    elif residual_out is not None:
+        raise ValueError("residual_out without a residual")
+    with _OnDevice(x.device) as s:
+        _check(lib.ternix_b200_rmsnorm_quantize(px, ldx, pr, ldr, codes[x.dtype], pw, w_dtype, eps, ph, ldh, out.data_ptr(),
+                                                row_scale.data_ptr(), M, K, s), "rmsnorm_quantize")
+    return (out, row_scale) if residual is None else (out, row_scale, residual_out)
+
+
+def glu_quantize(gate, up, activation: str = "silu", weight=None, eps=None, out=None, row_scale=None):
+    """The step between a gated feed-forward block's two products: z = act(gate) * up as int8 codes with one float32 scale
+    per row, in one pass on the current stream (ternix_b200_glu_quantize).  With `eps` the row is normalised first, z / rms(z) * weight.
+
+    gate, up: CUDA (M, K) of one type (bfloat16, float16 or float32), unit column stride, any row pitch, e.g. the two halves
+    of one product's output.  activation: "none", "relu", "relu2", "silu", "gelu" or "gelu_tanh".  weight: (K,) of the same
+    type or float32, only with eps.  Returns (codes, row_scale); rows of zeros and rows with an infinity or NaN as in
+    rmsnorm_quantize()."""
+    import torch
+
+    codes = _dtype_codes()
+    if not gate.is_cuda or gate.dim() != 2 or gate.dtype not in codes:
+        raise ValueError("glu_quantize takes CUDA (M, K) bfloat16, float16 or float32 tensors")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    if weight is not None and eps is None:
+        raise ValueError("a weight belongs to the norm: give eps too")
+    M, K = gate.shape
+    pg, ldg = _rows(gate, "gate", gate.device, gate.dtype, (M, K))
+    pu, ldu = _rows(up, "up", gate.device, gate.dtype, (M, K))
+    pw, w_dtype = None, 0
+    if weight is not None:
+        pw, w_dtype = _flat(weight, "weight", gate.device, (gate.dtype, torch.float32), K), codes.get(weight.dtype)
+    out, row_scale = _quantized_out(gate, out, row_scale)
+    with _OnDevice(gate.device) as s:
+        _check(lib.ternix_b200_glu_quantize(pg, ldg, pu, ldu, codes[gate.dtype], ACTIVATIONS[activation], eps is not None, pw,
+                                            w_dtype, 0.0 if eps is None else eps, out.data_ptr(), row_scale.data_ptr(), M, K, s),
+               "glu_quantize")
+    return out, row_scale
 
 
 class ProjectionGroup:

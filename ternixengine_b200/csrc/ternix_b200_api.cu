@@ -24,6 +24,7 @@
 #include "kernel_decode_mma.cuh"
 #include "kernel_gemv_group.cuh"
 #include "kernel_generic.cuh"
+#include "kernel_row_quant.cuh"
 #include "kernel_skinny_tc.cuh"
 
 namespace {
@@ -1126,6 +1127,46 @@ quantize_rows_kernel(const T* __restrict__ X, long long ldx, int8_t* __restrict_
         q = q > 127 ? 127 : q < -127 ? -127 : q;
         a[k] = static_cast<int8_t>(q);
     }
+}
+
+// ---------------------------------------------------------------- norm / gate + quantisation (kernel_row_quant.cuh)
+bool dtype_ok(int d) { return d == TERNIX_B200_DTYPE_F32 || d == TERNIX_B200_DTYPE_BF16 || d == TERNIX_B200_DTYPE_F16; }
+int dtype_bytes(int d) { return d == TERNIX_B200_DTYPE_F32 ? 4 : 2; }
+bool activation_ok(int a) { return a >= TERNIX_B200_ACT_NONE && a <= TERNIX_B200_ACT_GELU_TANH; }
+
+template <typename T, int MODE, int VPT, bool kVec>
+int launch_row_quant_t(const tb200::RowQuantArgs& p, int threads, cudaStream_t st) {
+    tb200::row_quant_kernel<T, MODE, VPT, kVec><<<p.M, threads, 0, st>>>(p);
+    TB_CUDA(cudaGetLastError());
+    return TERNIX_B200_OK;
+}
+
+template <typename T, int MODE>
+int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
+    constexpr int V = tb200::kRowVec<T>;
+    auto vec_ok = [&](const void* q, long long ld) { return !q || (aligned(q, 16) && (p.M == 1 || ld % V == 0)); };
+    const bool vec = p.K % V == 0 && vec_ok(p.x, p.ldx) && vec_ok(p.y, p.ldy) && vec_ok(p.h, p.ldh) && aligned(p.q, V) &&
+                     (!p.w || aligned(p.w, 16));
+    auto threads_for = [&](int items, int vpt) { return std::max(32, ((items + vpt - 1) / vpt + 31) / 32 * 32); };
+    if (vec) {
+        const int items = p.K / V;
+        if (items <= 512) return launch_row_quant_t<T, MODE, 1, true>(p, threads_for(items, 1), st);
+        if (items <= 1024) return launch_row_quant_t<T, MODE, 2, true>(p, threads_for(items, 2), st);
+        if (items <= 4096) return launch_row_quant_t<T, MODE, 4, true>(p, threads_for(items, 4), st);
+    } else {
+        if (p.K <= 4096) return launch_row_quant_t<T, MODE, 4, false>(p, threads_for(p.K, 4), st);
+        if (p.K <= 16384) return launch_row_quant_t<T, MODE, 16, false>(p, threads_for(p.K, 16), st);
+    }
+    tb200::row_quant_long_kernel<T, MODE><<<p.M, 1024, 0, st>>>(p);
+    TB_CUDA(cudaGetLastError());
+    return TERNIX_B200_OK;
+}
+
+template <int MODE>
+int launch_row_quant_dtype(int dtype, const tb200::RowQuantArgs& p, cudaStream_t st) {
+    if (dtype == TERNIX_B200_DTYPE_BF16) return launch_row_quant<__nv_bfloat16, MODE>(p, st);
+    if (dtype == TERNIX_B200_DTYPE_F16) return launch_row_quant<__half, MODE>(p, st);
+    return launch_row_quant<float, MODE>(p, st);
 }
 
 // y = bf16_rn((float(c) * row_scale[m]) * w_scale), from an int32 C to up to 8 bfloat16 destinations: the
@@ -2385,6 +2426,42 @@ int ternix_b200_quantize_rows(const void* dX, int x_dtype, long long ldx, int8_t
         quantize_rows_kernel<__nv_bfloat16><<<M, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(dX), ldx, dA, d_row_scale, M, K);
     TB_CUDA(cudaGetLastError());
     return TERNIX_B200_OK;
+}
+
+int ternix_b200_rmsnorm_quantize(const void* dX, long long ldx, const void* dResidual, long long ldr, int x_dtype,
+                                 const void* dWeight, int w_dtype, float eps, void* dH, long long ldh, int8_t* dA,
+                                 float* d_row_scale, int M, int K, void* stream) {
+    if (M < 0 || K < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!dtype_ok(x_dtype) || (dWeight && w_dtype != x_dtype && w_dtype != TERNIX_B200_DTYPE_F32)) return TERNIX_B200_ERR_INVALID_ARG;
+    if (!(eps >= 1e-12f && eps <= 1.0f)) return TERNIX_B200_ERR_INVALID_ARG;
+    if (M == 0) return TERNIX_B200_OK;
+    if (!d_row_scale || (K > 0 && (!dX || !dA)) || (!dResidual) != (!dH)) return TERNIX_B200_ERR_INVALID_ARG;
+    if (ldx < K || (dResidual && (ldr < K || ldh < K))) return TERNIX_B200_ERR_INVALID_ARG;
+    const uintptr_t e = static_cast<uintptr_t>(dtype_bytes(x_dtype));
+    if (!aligned(dX, e) || !aligned(dResidual, e) || !aligned(dH, e) || !aligned(d_row_scale, 4) ||
+        (dWeight && !aligned(dWeight, static_cast<uintptr_t>(dtype_bytes(w_dtype)))))
+        return TERNIX_B200_ERR_INVALID_ARG;
+    const tb200::RowQuantArgs p{dX, dResidual, dWeight, dH, dA, d_row_scale, ldx, ldr, ldh, M, K, eps, w_dtype, 0};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dResidual ? launch_row_quant_dtype<tb200::kRowNormResidual>(x_dtype, p, st)
+                     : launch_row_quant_dtype<tb200::kRowNorm>(x_dtype, p, st);
+}
+
+int ternix_b200_glu_quantize(const void* dGate, long long ldg, const void* dUp, long long ldu, int dtype, int activation,
+                             int norm, const void* dWeight, int w_dtype, float eps, int8_t* dA, float* d_row_scale, int M,
+                             int K, void* stream) {
+    if (M < 0 || K < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!dtype_ok(dtype) || !activation_ok(activation)) return TERNIX_B200_ERR_INVALID_ARG;
+    if (dWeight && (!norm || (w_dtype != dtype && w_dtype != TERNIX_B200_DTYPE_F32))) return TERNIX_B200_ERR_INVALID_ARG;
+    if (norm && !(eps >= 1e-12f && eps <= 1.0f)) return TERNIX_B200_ERR_INVALID_ARG;
+    if (M == 0) return TERNIX_B200_OK;
+    if (!d_row_scale || (K > 0 && (!dGate || !dUp || !dA)) || ldg < K || ldu < K) return TERNIX_B200_ERR_INVALID_ARG;
+    const uintptr_t e = static_cast<uintptr_t>(dtype_bytes(dtype));
+    if (!aligned(dGate, e) || !aligned(dUp, e) || !aligned(d_row_scale, 4) ||
+        (dWeight && !aligned(dWeight, static_cast<uintptr_t>(dtype_bytes(w_dtype)))))
+        return TERNIX_B200_ERR_INVALID_ARG;
+    const tb200::RowQuantArgs p{dGate, dUp, dWeight, nullptr, dA, d_row_scale, ldg, ldu, 0, M, K, norm ? eps : -1.0f, w_dtype, activation};
+    return launch_row_quant_dtype<tb200::kRowGate>(dtype, p, static_cast<cudaStream_t>(stream));
 }
 
 int ternix_b200_matmul_dequant(const int8_t* dA, const uint8_t* dW, void* const* dY_list, int n_dest,

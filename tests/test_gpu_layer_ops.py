@@ -1,0 +1,265 @@
+"""Norm and gate in front of the quantiser (rmsnorm_quantize, glu_quantize) on the GPU, against their CPU restatement: codes
+and the residual stream bit for bit wherever every operation is exactly rounded, scales within the bound of an fp32 sum."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+import ternixengine_b200 as tb
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "oracle"))
+import layer_ops_oracle as oracle  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["bfloat16", "float16", "float32"]
+# one element, less than a warp, whole vectors, odd lengths, every register form, beyond the registers of a CTA
+SHAPES = [(1, 1), (3, 7), (2, 64), (1, 2560), (5, 2561), (37, 4099), (7, 4104), (4, 8192), (3, 16392), (2, 16401), (2, 32768), (2, 40968)]
+
+
+def to_np(x):
+    return x.float().cpu().numpy()
+
+
+def make(shape, dtype, seed, scale=1.0):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows = torch.rand(shape[0], 1, generator=g, device="cuda") * 8 + 0.01
+    return (torch.randn(shape, generator=g, device="cuda") * rows * scale).to(getattr(torch, dtype))
+
+
+def check_quantized(codes, scale, t32, ms, eps, K):
+    """Codes equal the float32 restatement's bit for bit; scales within the bound, plus 2^-150: a float32 below 2^-126 is a
+    multiple of 2^-149, so rounding to one is off by up to half of that whatever its relative size."""
+    q, m = oracle.quantize(t32)
+    assert np.array_equal(codes.cpu().numpy(), q)
+    want = oracle.row_scale64(m, ms, eps)
+    got = scale.cpu().numpy().astype(np.float64)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    ok = ~np.isnan(want)
+    assert (np.abs(got[ok] - want[ok]) <= want[ok] * oracle.row_scale_bound(K) + 2.0 ** -150).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm_quantize(shape, dtype, residual):
+    import torch
+    M, K = shape
+    x = make(shape, dtype, M + K)
+    x[M - 1] = 0 if M > 1 else x[M - 1]
+    r = make(shape, dtype, M + K + 1, 3.0) if residual else None
+    if residual and M > 1:
+        r[M - 1] = 0
+    for weight in (None, (torch.randn(K, device="cuda") * 0.3 + 1).to(x.dtype), torch.randn(K, device="cuda") * 0.3 + 1):
+        got = tb.rmsnorm_quantize(x, weight, residual=r, eps=1e-5)
+        h = to_np(x)
+        if residual:
+            h_t = (x.float() + r.float()).to(x.dtype)
+            assert torch.equal(got[2], h_t)
+            h = to_np(h_t)
+        t = h if weight is None else (h * to_np(weight)[None, :]).astype(np.float32)
+        check_quantized(got[0], got[1], t, (h.astype(np.float64) ** 2).mean(axis=1), 1e-5, K)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", list(tb.ACTIVATIONS))
+def test_glu_quantize(shape, dtype, act):
+    """relu, relu2 and none: bit for bit.  The others: a code lies within half a step and the activation's error of the
+    exact quotient."""
+    import torch
+    M, K = shape
+    gu = torch.cat([make(shape, dtype, K, 0.5), make(shape, dtype, K + 7)], dim=1)
+    if M > 1:
+        gu[M - 1] = 0
+    gate, up = gu[:, :K], gu[:, K:]
+    g, u = to_np(gate), to_np(up)
+    for eps, weight in ((None, None), (1e-6, None), (1e-6, torch.randn(K, device="cuda") * 0.3 + 1)):
+        codes, scale = tb.glu_quantize(gate, up, activation=act, weight=weight, eps=eps)
+        w = np.ones(K, dtype=np.float32) if weight is None else to_np(weight)
+        if act in ("none", "relu", "relu2"):
+            a = g if act == "none" else np.where(g < 0, np.float32(0), g)
+            a = (a * a).astype(np.float32) if act == "relu2" else a
+            z = (a * u).astype(np.float32)
+            t = z if weight is None else (z * w).astype(np.float32)
+            check_quantized(codes, scale, t, (z.astype(np.float64) ** 2).mean(axis=1), eps, K)
+            continue
+        z = oracle.activate64(g, act) * u
+        t = z * w
+        # the activation's error, the roundings of act, act * up and * weight, and of the maximum
+        err = (oracle.activation_error(g, act) + 3 * np.abs(oracle.activate64(g, act)) * 2.0 ** -24) * np.abs(u * w)
+        m = np.abs(t).max(axis=1, keepdims=True)
+        m_err = (err * (np.abs(t) + 2 * err >= m)).max(axis=1, keepdims=True)
+        live = m[:, 0] > 0
+        with np.errstate(all="ignore"):
+            v = 127 * t / m
+            bound = 0.5 + 127 * (err + np.abs(t) * m_err / m) / m + 127 * 3 * 2.0 ** -24
+        q = codes.cpu().numpy().astype(np.float64)
+        assert (np.abs(q - v)[live] <= bound[live]).all() and (q[~live] == 0).all()
+        want = oracle.row_scale64(m[:, 0], (z ** 2).mean(axis=1), eps)
+        # a norm's sum is off by at most twice the largest weighed error of its terms
+        z_err = 2 * (err / np.maximum(np.abs(w), 1e-30) * np.abs(z)).sum(axis=1) / np.maximum((z ** 2).sum(axis=1), 1e-300)
+        with np.errstate(all="ignore"):
+            rel = oracle.row_scale_bound(K) + m_err[:, 0] / m[:, 0] + (0 if eps is None else z_err)
+        got = scale.cpu().numpy().astype(np.float64)
+        assert (np.abs(got - want)[live] <= (want * rel)[live]).all() and (got[~live] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", [2560, 2561, 40968])
+def test_rows_that_are_not_ordinary(dtype, K):
+    """Zeros, infinities, NaN, the type's lowest and smallest values, a sum of squares that leaves fp32, a single value."""
+    import torch
+    t = getattr(torch, dtype)
+    info = torch.finfo(t)
+    x = make((10, K), dtype, 5)
+    x[0] = 0
+    x[1, K // 2] = float("inf")
+    x[2, K - 1] = float("-inf")
+    x[3, 3] = float("nan")
+    x[4] = info.min                              # float16: 65504^2 x K still fits fp32; the others overflow
+    x[5] = info.smallest_normal * 2
+    x[6] = 0
+    x[6, K - 1] = -3.0
+    x[7, 0] = float("inf")
+    x[7, 1] = float("nan")
+    x[8] = 0
+    x[8, 5] = info.smallest_normal * info.eps if dtype == "float32" else info.smallest_normal     # smallest of all
+    codes, scale = tb.rmsnorm_quantize(x, eps=1e-5)
+    q, s = codes.cpu().numpy(), scale.cpu().numpy()
+    bad = [1, 2, 3, 7] + ([4] if dtype != "float16" else [])
+    assert (q[bad] == 0).all() and np.isnan(s[bad]).all()
+    good = [i for i in range(10) if i not in bad]
+    h = to_np(x)[good]
+    check_quantized(codes[good], scale[good], h, (h.astype(np.float64) ** 2).mean(axis=1), 1e-5, K)
+    assert s[0] == 1 and (q[5] == 127).all() and q[6, K - 1] == -127 and q[8, 5] == 127
+    # the same rows as a gate's second factor: finite rows as before, the others poisoned, nothing spills into a neighbour
+    one = torch.ones_like(x)
+    cg, sg = tb.glu_quantize(one, x, activation="relu")
+    bad = [1, 2, 3, 7]
+    assert (cg.cpu().numpy()[bad] == 0).all() and np.isnan(sg.cpu().numpy()[bad]).all()
+    good = [i for i in range(10) if i not in bad]
+    check_quantized(cg[good], sg[good], to_np(x)[good], None, None, K)
+
+
+def test_residual_in_place_and_pitches():
+    """residual_out may be the residual or x; rows may have any pitch and start anywhere; what lies around stays.  Codes and
+    h are the same bits; a scale may differ by twice its bound, because rows that a 16-byte load cannot address are spread
+    over the threads in another order and each order's sum is within the bound of the exact one."""
+    import torch
+
+    def same(got, want):
+        tol = 2 * oracle.row_scale_bound(got[0].shape[1])
+        return torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and \
+            bool(((got[1].double() - want[1].double()).abs() <= want[1].double() * tol).all())
+
+    for dtype in (torch.bfloat16, torch.float32):
+        for K, off, pad in ((2560, 0, 16), (2560, 3, 5), (130, 1, 2), (40970, 2, 6)):
+            M = 6
+            wide = torch.randn(M + 2, K + off + pad, device="cuda").to(dtype)
+            res = torch.randn(M, K + pad, device="cuda").to(dtype)
+            keep_w, keep_r = wide.clone(), res.clone()
+            x, r = wide[1:M + 1, off:off + K], res[:, :K]
+            want = tb.rmsnorm_quantize(x.contiguous(), residual=r.contiguous())
+            got = tb.rmsnorm_quantize(x, residual=r)
+            assert same(got, want)
+            got = tb.rmsnorm_quantize(x, residual=r, residual_out=r)
+            assert same(got, want) and got[2] is r
+            assert torch.equal(res[:, K:], keep_r[:, K:]) and torch.equal(wide, keep_w)
+            res.copy_(keep_r)
+            got = tb.rmsnorm_quantize(x, residual=r, residual_out=x)
+            assert same(got, want)
+            wide[1:M + 1, off:off + K] = keep_w[1:M + 1, off:off + K]
+            assert torch.equal(wide, keep_w) and torch.equal(res, keep_r)
+
+
+def test_outputs_of_the_caller_and_empty_sizes():
+    import torch
+    x = make((9, 640), "bfloat16", 1)
+    codes = torch.full((12, 640), 55, dtype=torch.int8, device="cuda")
+    scale = torch.full((12,), 7.0, device="cuda")
+    want = tb.rmsnorm_quantize(x)
+    got = tb.rmsnorm_quantize(x, out=codes[:9], row_scale=scale[:9])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert (codes[9:] == 55).all() and (scale[9:] == 7).all()
+    empty = torch.empty((0, 640), dtype=torch.bfloat16, device="cuda")
+    q, s = tb.rmsnorm_quantize(empty)
+    assert q.shape == (0, 640) and s.shape == (0,)
+    q, s = tb.rmsnorm_quantize(torch.empty((3, 0), dtype=torch.float32, device="cuda"))
+    assert q.shape == (3, 0) and (s == 1).all()
+    q, s, h = tb.rmsnorm_quantize(empty, residual=empty)
+    assert h.shape == (0, 640)
+    assert tb.glu_quantize(empty, empty)[0].shape == (0, 640)
+
+
+def test_rows_past_32_bit_offsets():
+    """Element offsets beyond 2^31 in the inputs and byte offsets beyond 2^31 in the codes."""
+    import torch
+    M, K = 66000, 32768
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device="cuda")
+    rows = [0, 65535, 65536, M - 1]
+    x[rows] = make((4, K), "bfloat16", 3)
+    codes, scale = tb.rmsnorm_quantize(x)
+    h = to_np(x[rows])
+    check_quantized(codes[rows], scale[rows], h, (h.astype(np.float64) ** 2).mean(axis=1), 1e-5, K)
+    assert (codes[1:65535:977] == 0).all() and (scale[1:65535] == 1).all()
+
+
+def test_streams_and_graphs():
+    """On another stream, and captured once and replayed on new inputs."""
+    import torch
+    x, r = make((33, 2560), "bfloat16", 1), make((33, 2560), "bfloat16", 2)
+    w = torch.randn(2560, device="cuda").to(torch.bfloat16)
+    want = tb.rmsnorm_quantize(x, w, residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = tb.rmsnorm_quantize(x, w, residual=r)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a = tb.rmsnorm_quantize(x, w, residual=r)
+        b = tb.glu_quantize(x, a[2], activation="silu", weight=w, eps=1e-5)
+    for seed in (11, 12):
+        x.copy_(make((33, 2560), "bfloat16", seed))
+        g.replay()
+        want = tb.rmsnorm_quantize(x, w, residual=r)
+        want2 = tb.glu_quantize(x, want[2], activation="silu", weight=w, eps=1e-5)
+        assert all(torch.equal(p, q) for p, q in zip(a, want)) and all(torch.equal(p, q) for p, q in zip(b, want2))
+
+
+def test_refusals():
+    import torch
+    x = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda")
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    bad = [
+        lambda: tb.rmsnorm_quantize(x.cpu()),
+        lambda: tb.rmsnorm_quantize(x.double()),
+        lambda: tb.rmsnorm_quantize(x[0]),
+        lambda: tb.rmsnorm_quantize(x.t()),
+        lambda: tb.rmsnorm_quantize(x[:1].expand(4, 64)),
+        lambda: tb.rmsnorm_quantize(x, w[:63]),
+        lambda: tb.rmsnorm_quantize(x, w.half()),
+        lambda: tb.rmsnorm_quantize(x, w.cpu()),
+        lambda: tb.rmsnorm_quantize(x, residual=x.float()),
+        lambda: tb.rmsnorm_quantize(x, residual=x[:3]),
+        lambda: tb.rmsnorm_quantize(x, residual_out=x),
+        lambda: tb.rmsnorm_quantize(x, eps=0.0),
+        lambda: tb.rmsnorm_quantize(x, eps=float("nan")),
+        lambda: tb.rmsnorm_quantize(x, eps=2.0),
+        lambda: tb.rmsnorm_quantize(x, out=torch.empty((4, 64), dtype=torch.uint8, device="cuda")),
+        lambda: tb.rmsnorm_quantize(x, out=torch.empty((4, 128), dtype=torch.int8, device="cuda")[:, :64]),
+        lambda: tb.rmsnorm_quantize(x, row_scale=torch.empty(3, device="cuda")),
+        lambda: tb.glu_quantize(x, x, activation="swish"),
+        lambda: tb.glu_quantize(x, x, weight=w),
+        lambda: tb.glu_quantize(x, x.half()),
+        lambda: tb.glu_quantize(x, x[:, :32]),
+        lambda: tb.glu_quantize(x, x, eps=0.0),
+        lambda: tb.glu_quantize(x.cpu(), x.cpu()),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
