@@ -289,6 +289,30 @@ int ternix_b200_glu_quantize(const void *dGate, long long ldg, const void *dUp, 
                              int norm, const void *dWeight, int w_dtype, float eps, int8_t *dA, float *d_row_scale, int M,
                              int K, void *stream);
 
+/* The product with the rest of the linear step in its epilogue; the int32 sums stay on chip:
+ *   y[m,n] = T( act( (float(c[m,n]) * row_scale[m]) * scale[n] + bias[n] ) + residual[m,n] ),  c the exact int32 product,
+ * in fp32, every operation rounded on its own and in this order, one rounding to the output's type T at the end; the
+ * result is the same whichever kernel runs.  scale[n] is col_scale[n], or w_scale for all columns where col_scale is
+ * NULL (column scales let projections with scales of their own share one weight matrix).  bias and residual may be NULL;
+ * bias is [N] of bias_dtype; residual has the output's type and row pitch ldr >= N and may be dY itself (not a shifted
+ * view of it).  dY has row pitch ldy >= N.  Sums beyond 2^24 (|c| can reach 128 K) round once on their way to fp32.
+ * Shapes, alignment, `kernel` and d_status as in ternix_b200_matmul_ex; GEMM_TC is the tensor-memory kernel.  K == 0 gives
+ * y = act(bias) + residual.  A product with a ragged K, N or unaligned operand that is too large for the generic kernel
+ * takes an aligned copy of its operands from the library's pool (ternix_b200_release_cached_memory), on `stream`. */
+typedef struct ternix_b200_epilogue {
+    const float *row_scale;    /* [M] */
+    const float *col_scale;    /* [N] or NULL */
+    float w_scale;             /* used where col_scale is NULL */
+    int activation;            /* TERNIX_B200_ACT_* */
+    const void *bias;
+    int bias_dtype;
+    int out_dtype;             /* TERNIX_B200_DTYPE_* of dY and residual */
+    const void *residual;
+    long long ldr;
+} ternix_b200_epilogue;
+int ternix_b200_matmul_fused(const int8_t *dA, const uint8_t *dW, const ternix_b200_epilogue *epilogue, void *dY,
+                             long long ldy, int M, int K, int N, int kernel, int32_t *d_status, void *stream);
+
 /* ---- N-column sharding plan (host arithmetic only) ---------------------------------------------
  * Splits N columns over `world` ranks in granules of `granule` columns (a multiple of 4; 64 keeps each
  * shard's packed rows 16-byte aligned).  Writes the first column and the column count of `rank`.

@@ -11,7 +11,7 @@ import math
 import numpy as np
 
 F = np.float32
-_ERF = np.vectorize(math.erf, otypes=[np.float64])
+_ERFC = np.vectorize(math.erfc, otypes=[np.float64])
 
 
 def activate64(v, act):
@@ -25,9 +25,10 @@ def activate64(v, act):
         if act == "silu":
             return v / (1 + np.exp(-v))
         if act == "gelu":
-            return v * (1 + _ERF(v / math.sqrt(2))) / 2
+            return v * _ERFC(-v / math.sqrt(2)) / 2                 # 1 + erf(x) = erfc(-x), without the cancellation
         if act == "gelu_tanh":
-            return v * (1 + np.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3))) / 2
+            # (1 + tanh u) / 2 = 1 / (1 + exp(-2u)), without the cancellation
+            return v / (1 + np.exp(-2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)))
     return v
 
 
@@ -37,16 +38,17 @@ def activation_error(v, act):
     relu and relu2 are exactly rounded.  silu = v / (1 + e), e = exp(-v) from the hardware's exponential: its documented
     error is 2 + 1.173 |v| units in the last place (2^-23), the sum rounds once (2^-24) and the quotient has 2 ulp, so the
     result is off by at most its own size x (2 + 1.173 |v| + 3) x 2^-23.  gelu_tanh is the same with the argument 2u, which
-    itself carries four roundings (4 |2u| 2^-24 in the exponent).  gelu = 0.5 v (1 + erf): erff has 2 ulp and its argument
+    itself carries four roundings (4 |2u| 2^-24 in the exponent).  Both divide with the instruction that delivers 0 for
+    denominators above 2^126 (documented), where the quotient is at most |v| 2^-126.  gelu = 0.5 v (1 + erf): erff has 2 ulp and its argument
     one rounding and a rounded constant (|d erf| <= 1.13 |x| 2^-23 <= 2^-23 where erf still moves), the sum one rounding of
     a value up to 2: in all |v| (2 x 2^-24 + 2^-23 + 2 x 2^-24) / 2, and two roundings of the products."""
     v = np.asarray(v, dtype=np.float64)
     out = np.abs(activate64(v, act))
     if act == "silu":
-        return out * (5 + 1.173 * np.abs(v)) * 2.0 ** -23
+        return out * (5 + 1.173 * np.abs(v)) * 2.0 ** -23 + np.abs(v) * 2.0 ** -126
     if act == "gelu_tanh":
         u2 = 2 * math.sqrt(2 / math.pi) * np.abs(v + 0.044715 * v ** 3)
-        return out * (5 + 3.173 * u2) * 2.0 ** -23
+        return out * (5 + 3.173 * u2) * 2.0 ** -23 + np.abs(v) * 2.0 ** -126
     if act == "gelu":
         return np.abs(v) * 2.0 ** -23 * 1.5 + out * 2.0 ** -23
     return np.zeros_like(v)

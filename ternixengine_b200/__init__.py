@@ -55,7 +55,7 @@ EXPORTS = (
     "ternix_b200_prepack_k4", "ternix_b200_prepack_k4_bytes", "ternix_b200_group_run", "ternix_b200_group_launches", "ternix_b200_group_destroy",
     "ternix_b200_gemv_batch_noalloc", "ternix_b200_gemv_batch_noalloc_limits",
     "ternix_b200_quantize_rows", "ternix_b200_matmul_dequant",
-    "ternix_b200_rmsnorm_quantize", "ternix_b200_glu_quantize",
+    "ternix_b200_rmsnorm_quantize", "ternix_b200_glu_quantize", "ternix_b200_matmul_fused",
     "ternix_b200_matmul_bcast", "ternix_b200_peer_alloc", "ternix_b200_peer_free", "ternix_b200_peer_export",
     "ternix_b200_peer_import", "ternix_b200_peer_close", "ternix_b200_peer_barrier",
     "ternix_b200_shard_columns", "ternix_b200_unpack_gathered",
@@ -67,6 +67,13 @@ class _Problem(ctypes.Structure):
     """struct ternix_b200_problem"""
     _fields_ = [("dA", ctypes.c_void_p), ("dW", ctypes.c_void_p), ("dC", ctypes.c_void_p),
                 ("M", ctypes.c_int), ("K", ctypes.c_int), ("N", ctypes.c_int), ("ldc", ctypes.c_longlong)]
+
+
+class _Epilogue(ctypes.Structure):
+    """struct ternix_b200_epilogue"""
+    _fields_ = [("row_scale", ctypes.c_void_p), ("col_scale", ctypes.c_void_p), ("w_scale", ctypes.c_float),
+                ("activation", ctypes.c_int), ("bias", ctypes.c_void_p), ("bias_dtype", ctypes.c_int),
+                ("out_dtype", ctypes.c_int), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_longlong)]
 
 
 class TernixError(RuntimeError):
@@ -120,6 +127,7 @@ def _load() -> ctypes.CDLL:
         "ternix_b200_quantize_rows": (i32, [vp, i32, i64, vp, vp, i32, i32, vp]),
         "ternix_b200_rmsnorm_quantize": (i32, [vp, i64, vp, i64, i32, vp, i32, c.c_float, vp, i64, vp, vp, i32, i32, vp]),
         "ternix_b200_glu_quantize": (i32, [vp, i64, vp, i64, i32, i32, i32, vp, i32, c.c_float, vp, vp, i32, i32, vp]),
+        "ternix_b200_matmul_fused": (i32, [vp, vp, c.POINTER(_Epilogue), vp, i64, i32, i32, i32, i32, vp, vp]),
         "ternix_b200_matmul_dequant": (i32, [vp, vp, c.POINTER(vp), i32, vp, c.c_float, i32, i32, i32, i64, vp, vp]),
         "ternix_b200_matmul_bcast": (i32, [vp, vp, c.POINTER(vp), i32, i32, i32, i32, i64, vp, vp]),
         "ternix_b200_peer_alloc": (i32, [c.POINTER(vp), sz]),
@@ -535,6 +543,58 @@ def glu_quantize(gate, up, activation: str = "silu", weight=None, eps=None, out=
                                             w_dtype, 0.0 if eps is None else eps, out.data_ptr(), row_scale.data_ptr(), M, K, s),
                "glu_quantize")
     return out, row_scale
+
+
+def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str = "none", residual=None, out=None,
+                 out_dtype=None, kernel: str = "auto", status=None):
+    """y = act((A x W) * row_scale[:, None] * w_scale + bias) + residual with the integer product exact, everything behind
+    it in float32 in the kernel's epilogue and one rounding at the end, on the current stream (ternix_b200_matmul_fused).
+
+    a: CUDA (M, K) int8, w_packed: (K, N/4) uint8, both contiguous.  row_scale: (M,) float32, as the quantisers return it.
+    w_scale: a number, or an (N,) float32 tensor.  bias: (N,) float32, bfloat16 or float16.  activation: "none", "relu",
+    "relu2", "silu", "gelu" or "gelu_tanh".  residual: (M, N) of the output's type, unit column stride, any row pitch; may be
+    `out` itself.  out: (M, N) bfloat16, float16 or float32, unit column stride, any row pitch; without it a new tensor of
+    out_dtype (the residual's type, else bfloat16)."""
+    import torch
+
+    codes = _dtype_codes()
+    if not (a.is_cuda and w_packed.is_cuda):
+        raise ValueError("matmul_fused() takes CUDA tensors")
+    if a.dtype != torch.int8 or w_packed.dtype != torch.uint8 or a.dim() != 2 or w_packed.dim() != 2:
+        raise ValueError("A must be (M, K) int8 and W_packed (K, N/4) uint8")
+    if w_packed.device != a.device:
+        raise ValueError("A and W_packed must be on one device")
+    if not (a.is_contiguous() and w_packed.is_contiguous()):
+        raise ValueError("A and W_packed must be contiguous")
+    M, K = a.shape
+    if w_packed.shape[0] != K:
+        raise ValueError("inner dimensions do not match")
+    N = w_packed.shape[1] * 4
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    if kernel not in KERNELS:
+        raise ValueError(f"kernel must be one of {', '.join(KERNELS)}")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype or (torch.bfloat16 if residual is None else residual.dtype), device=a.device)
+    elif out_dtype is not None and out_dtype != out.dtype:
+        raise ValueError("out has another type than out_dtype")
+    if out.dtype not in codes:
+        raise ValueError("the output is bfloat16, float16 or float32")
+    py, ldy = _rows(out, "out", a.device, out.dtype, (M, N))
+    ep = _Epilogue(row_scale=_flat(row_scale, "row_scale", a.device, (torch.float32,), M), activation=ACTIVATIONS[activation],
+                   out_dtype=codes[out.dtype])
+    if isinstance(w_scale, torch.Tensor):
+        ep.col_scale = _flat(w_scale, "w_scale", a.device, (torch.float32,), N)
+    else:
+        ep.w_scale = w_scale
+    if bias is not None:
+        ep.bias, ep.bias_dtype = _flat(bias, "bias", a.device, codes, N), codes.get(bias.dtype, 0)
+    if residual is not None:
+        ep.residual, ep.ldr = _rows(residual, "residual", a.device, out.dtype, (M, N))
+    with _OnDevice(a.device) as s:
+        _check(lib.ternix_b200_matmul_fused(a.data_ptr(), w_packed.data_ptr(), ctypes.byref(ep), py, ldy, M, K, N, KERNELS[kernel],
+                                            status.data_ptr() if status is not None else None, s), "matmul_fused")
+    return out
 
 
 class ProjectionGroup:

@@ -126,11 +126,12 @@ __device__ __forceinline__ int mma_item_tiles(const MmaItem& it, int K) {
 // The 16-byte group (4 columns of one batch row) that accumulator registers (ng, rr, bp, hh) of a lane make up:
 // batch row 8 ng + 2 (lane % 4) + rr of the row group, byte column 16 bp + 8 hh + lane / 4 of the warp's block.
 // Groups are numbered p = ((ng * 2 + rr) * 2 + bp) * 2 + hh.
-template <bool kSingle, int NG>
+template <bool kSingle, int NG, typename Epi = StoreInt32>
 __global__ void __launch_bounds__(kMmaThreads, kMmaCtasPerSm)
 ternary_decode_mma_kernel(const __grid_constant__ MmaProblem single, const MmaSingle sg,
                           const MmaProblem* __restrict__ probs, const MmaItem* __restrict__ items,
-                          const int* __restrict__ cta_first, int32_t* __restrict__ status) {
+                          const int* __restrict__ cta_first, int32_t* __restrict__ status, const Epi epi) {
+    static_assert(kSingle || !Epi::kFused, "the fused epilogue is built for single products");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* stages = base;
@@ -288,7 +289,9 @@ ternary_decode_mma_kernel(const __grid_constant__ MmaProblem single, const MmaSi
                             int32_t v[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) v[j] = (acc[bp][j][ng][2 * hh + rr] >> (2 * j)) - corr;
-                            if (add) {
+                            if constexpr (Epi::kFused) {
+                                epi.store4(row, col, v);
+                            } else if (add) {
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) atomicAdd(crow + col + q, v[q]);
                             } else if (p->c_vec_ok) {
@@ -324,17 +327,27 @@ ternary_decode_mma_kernel(const __grid_constant__ MmaProblem single, const MmaSi
                 const int row = (it.row0 & 0xffff) + 8 * ng + 2 * (lane & 3) + rr;
                 const int col = it.chunk * kMmaItemCols + warp * 128 + (16 * bp + 8 * hh + (lane >> 2)) * 4;
                 if (row < single.M && col < single.N) {
-                    int32_t* dst = single.C + static_cast<size_t>(row) * single.ldc + col;
-                    if (single.c_vec_ok) {
-                        *reinterpret_cast<int4*>(dst) = make_int4(v[0], v[1], v[2], v[3]);
+                    if constexpr (Epi::kFused) {
+                        epi.store4(row, col, v);
                     } else {
+                        int32_t* dst = single.C + static_cast<size_t>(row) * single.ldc + col;
+                        if (single.c_vec_ok) {
+                            *reinterpret_cast<int4*>(dst) = make_int4(v[0], v[1], v[2], v[3]);
+                        } else {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) dst[x] = v[x];
+                            for (int x = 0; x < 4; ++x) dst[x] = v[x];
+                        }
                     }
                 }
             }
         }
-        cluster_sync_all();        // nobody leaves while a peer may still read its shared memory
+        // nobody leaves while a peer may still read its shared memory
+        if constexpr (Epi::kFused) {
+            __syncwarp();
+            cluster_sync_threads();       // the epilogue may have parted a warp's lanes
+        } else {
+            cluster_sync_all();
+        }
     }
     if (tid == 0 && *abort_flag && status) atomicMax(status, kStatusTimeout);
 }

@@ -56,6 +56,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cstdint>
+#include "epilogue.cuh"
 #include "kernel_gemm_tc2.cuh"
 
 namespace tb200 {
@@ -269,14 +270,18 @@ __device__ __forceinline__ void sts_u16(uint32_t saddr, uint16_t v) {
 // pair's MMAs are half as long, and tensor-memory columns 0-255 hold TWO accumulators: the MMAs of the next tile run
 // while the epilogue warps empty the previous one.  The shared-memory ring is then deeper than the operand ring in
 // tensor memory (a stage passes in half the time, the latency of a TMA load stays what it is).
-template <bool kGrouped, bool kBf16 = false, int TA = kTc3TileA>
+// Epi = FusedEpilogue: the finished sums go through the staging buffer as int32, and the four warps of an epilogue group
+// read it back row by row, four columns to a lane: scales, bias, activation and residual in registers, coalesced loads of
+// the residual and stores of the output (256 bytes of bfloat16 per row and warp) at any pitch, without a TMA view.
+template <bool kGrouped, bool kBf16 = false, int TA = kTc3TileA, typename Epi = StoreInt32>
 __global__ void __launch_bounds__(kTc3Threads, 1)
 ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                         const __grid_constant__ Tc3Stores stores, int32_t* __restrict__ C, int M, int K, int N,
                         long long ldc, const Tc3Problem* __restrict__ probs, const Tc2Tile* __restrict__ tiles,
                         const int* __restrict__ pair_first, int32_t* __restrict__ status,
-                        const float* __restrict__ row_scale = nullptr, float w_scale = 1.0f) {
-    static_assert(!(kGrouped && kBf16), "the dequantising epilogue is built for single products");
+                        const float* __restrict__ row_scale, float w_scale, const Epi epi) {
+    static_assert(!(kGrouped && (kBf16 || Epi::kFused)) && !(kBf16 && Epi::kFused),
+                  "the dequantising and the fused epilogue are built for single products");
     using G = Tc3Geom<TA>;
     constexpr int kRowsPerCta = G::kRowsPerCta;                            // activation rows a CTA loads per stage
     constexpr uint32_t kStageTx = G::kStageBytes;                          // bytes a stage's TMA loads deliver
@@ -561,6 +566,33 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 if (elected) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kTc3EpiBufs - 1) : "memory");
                 asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
                 const int row0 = a_t * TA + 32 * c;
+                if constexpr (Epi::kFused) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        sts_u32(buf + ((j * 128 + colp) << 2), static_cast<uint32_t>(static_cast<int32_t>(r[i][j]) >> 6));
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
+                    const int col = col0 + 4 * lane;
+                    if (col < N) {
+                        float cs[4], b[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) { cs[x] = epi.column_scale(col + x); b[x] = epi.column_bias(col + x); }
+                        const int first = row0 + 8 * static_cast<int>(q), rows = min(8, M - first);
+#pragma unroll 2
+                        for (int j = 0; j < rows; ++j) {
+                            const uint4 raw = epi.load_residual4(first + j, col);
+                            const uint4 sum = lds_v4(buf + ((8 * q + j) * 128 + 4 * lane) * 4);
+                            const float rs = __ldg(epi.row_scale + first + j);
+                            float v[4] = {epi.linear(static_cast<int32_t>(sum.x), rs, cs[0], b[0]),
+                                          epi.linear(static_cast<int32_t>(sum.y), rs, cs[1], b[1]),
+                                          epi.linear(static_cast<int32_t>(sum.z), rs, cs[2], b[2]),
+                                          epi.linear(static_cast<int32_t>(sum.w), rs, cs[3], b[3])};
+                            activate(epi.act, v);
+                            epi.finish4(first + j, col, v, raw);
+                        }
+                    }
+                    __syncwarp();
+                    continue;
+                }
                 if constexpr (kBf16) {
                     // in place: r[i][j] becomes the bfloat16 bit pattern of the scaled value
 #pragma unroll

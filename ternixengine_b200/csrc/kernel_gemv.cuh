@@ -22,6 +22,7 @@
 #pragma once
 #include <cuda.h>
 #include <cstdint>
+#include "epilogue.cuh"
 #include "ptx_sm100.cuh"
 
 namespace tb200 {
@@ -46,11 +47,11 @@ constexpr size_t gemv_smem_bytes(int krange) {
            size_t(MR) * 16 * (WORDS + 1) * 4 + 2 * kGemvStages * 8 + 16;
 }
 
-template <int MR, int WORDS>
+template <int MR, int WORDS, typename Epi = StoreInt32>
 __global__ void __launch_bounds__(kGemvThreads)
 ternary_gemv_kernel(const __grid_constant__ CUtensorMap tmap_w, const int8_t* __restrict__ A,
                     int32_t* __restrict__ C, int M, int K, int N, long long ldc, int krange, int a_words_ok,
-                    int32_t* __restrict__ status) {
+                    int32_t* __restrict__ status, const Epi epi) {
     using G = GemvGeom<WORDS>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
@@ -209,10 +210,19 @@ ternary_gemv_kernel(const __grid_constant__ CUtensorMap tmap_w, const int8_t* __
 #pragma unroll
             for (uint32_t p = 0; p < 8; ++p) sum += v[p];
             const int grow = row0 + r, gcol = n_chunk * G::kCols + col;
-            if (grow < M && gcol < N) C[static_cast<size_t>(grow) * ldc + gcol] = sum >> 6;
+            if (grow < M && gcol < N) {
+                if constexpr (Epi::kFused) epi.store(grow, gcol, sum >> 6);
+                else C[static_cast<size_t>(grow) * ldc + gcol] = sum >> 6;
+            }
         }
     }
-    cluster_sync_all();   // nobody leaves while a peer may still read its shared memory
+    // nobody leaves while a peer may still read its shared memory
+    if constexpr (Epi::kFused) {
+        __syncwarp();
+        cluster_sync_threads();       // the epilogue may have parted a warp's lanes
+    } else {
+        cluster_sync_all();
+    }
 }
 
 }  // namespace tb200

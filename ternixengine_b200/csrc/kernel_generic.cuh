@@ -11,6 +11,8 @@
 // over blockIdx.z; the slices then add into a C that the host has zeroed (integer adds: still exact).
 #pragma once
 #include <cstdint>
+#include "epilogue.cuh"
+#include "ptx_sm100.cuh"
 
 namespace tb200 {
 
@@ -100,6 +102,127 @@ ternary_generic_kernel(const int8_t* __restrict__ A, const uint8_t* __restrict__
                 }
             }
         }
+    }
+}
+
+// The same shapes and alignments with the fused epilogue.  Byte loads as above, but a packed byte column of four
+// consecutive k-rows is put into one word while it is staged, so that a field of it is one shift and mask away from a
+// dp4a operand (0, +64, -64 as int8, as in the one-row kernel): 29 instructions per 64 products and thread instead of 120.
+// The sums are 64 times too large and are taken down (exactly) every kGenFlush k-rows, so K stays unbounded.
+// K is not cut between CTAs: a product large enough to want that is served by an aligned copy and the kernels behind it.
+constexpr int kGenFlush = 131072;      // 64 * 128 * 131072 = 2^30
+static_assert(kGenFlush % kGenK == 0, "flushes fall between slabs");
+
+template <typename Epi>
+__global__ void __launch_bounds__(kGenThreads)
+ternary_generic_fused_kernel(const int8_t* __restrict__ A, const uint8_t* __restrict__ W, int M, int K, int N, const Epi epi) {
+    __shared__ __align__(16) uint32_t sA[kGenRows][kGenK / 4];
+    __shared__ uint32_t sW[kGenK / 4][kGenBytes];
+
+    const int tid = threadIdx.x, tx = tid & 31, ty = tid >> 5;
+    const int pitch = N >> 2;
+    const int row0 = blockIdx.y * kGenRows, byte0 = blockIdx.x * kGenBytes;
+
+    int32_t acc[4][4] = {}, total[4][4] = {};
+    const int a_row = tid >> 3, a_k = (tid & 7) * 8;
+    int since = 0;
+    for (int k0 = 0; k0 < K; k0 += kGenK) {
+        {
+            const int8_t* src = A + static_cast<size_t>(row0 + a_row) * K + k0 + a_k;
+            uint32_t w[2] = {0, 0};
+            if (row0 + a_row < M) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k0 + a_k + i < K) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(src[i])) << (8 * (i & 3));
+            }
+            sA[a_row][a_k / 4] = w[0];
+            sA[a_row][a_k / 4 + 1] = w[1];
+#pragma unroll
+            for (int g = ty; g < kGenK / 4; g += kGenThreads / 32) {
+                uint32_t t = 0;
+                if (byte0 + tx < pitch) {
+                    const uint8_t* col = W + static_cast<size_t>(k0 + 4 * g) * pitch + byte0 + tx;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (k0 + 4 * g + i < K) t |= static_cast<uint32_t>(col[static_cast<size_t>(i) * pitch]) << (8 * i);
+                }
+                sW[g][tx] = t;
+            }
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int g = 0; g < kGenK / 4; ++g) {
+            const uint32_t t = sW[g][tx];
+            int a4[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a4[r] = static_cast<int>(sA[ty * 4 + r][g]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int x = static_cast<int>((t << (6 - 2 * c)) & 0xC0C0C0C0u);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[r][c] = __dp4a(x, a4[r], acc[r][c]);
+            }
+        }
+        __syncthreads();
+        since += kGenK;
+        if (since == kGenFlush) {
+            since = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) { total[r][c] += acc[r][c] >> 6; acc[r][c] = 0; }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) total[r][c] += acc[r][c] >> 6;
+
+    const int col = (byte0 + tx) * 4;
+    if (col < N) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (row0 + ty * 4 + r < M) epi.store4(row0 + ty * 4 + r, col, total[r]);
+    }
+}
+
+// Rows of `width` bytes at any address and pitch, copied to rows at a pitch (and base) of 16 bytes, which is what the TMA
+// unit can describe.  A thread writes 16 bytes and reads them as aligned words; a word that is not wholly inside the
+// source is put together from its bytes.  What lies between the width and the pitch is zeroed.
+__global__ void __launch_bounds__(256)
+align_rows_kernel(const uint8_t* __restrict__ src, long long src_pitch, uint8_t* __restrict__ dst, int dst_pitch, int width,
+                  long long rows) {
+    const int per_row = dst_pitch / 16;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(src);
+    const uintptr_t hi = lo + static_cast<uintptr_t>(rows - 1) * src_pitch + width;
+    const long long total = rows * per_row;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+        const long long r = i / per_row;
+        const int x = static_cast<int>(i - r * per_row) * 16;
+        const uintptr_t at = lo + static_cast<uintptr_t>(r) * src_pitch + x, word = at & ~uintptr_t(3);
+        const int shift = static_cast<int>(at & 3) * 8;
+        uint32_t w[5];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) {
+            const uintptr_t p = word + 4 * j;
+            w[j] = 0;
+            if (x + 4 * j - shift / 8 >= width) continue;
+            if (p >= lo && p + 4 <= hi) {
+                w[j] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    if (p + b >= lo && p + b < hi) w[j] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(p + b)) << (8 * b);
+            }
+        }
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[j] = __funnelshift_r(w[j], w[j + 1], shift);
+            const int left = width - x - 4 * j;             // bytes of this word that belong to the row
+            if (left < 4) o[j] &= left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+        }
+        *reinterpret_cast<uint4*>(dst + r * dst_pitch + x) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 

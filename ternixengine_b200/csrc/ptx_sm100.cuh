@@ -217,6 +217,10 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same for warps whose lanes may have parted: every thread arrives for itself.
+__device__ __forceinline__ void cluster_sync_threads() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
 // Address of `smem_addr` (a shared::cta address of this CTA's layout) inside CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t dsmem_map(uint32_t smem_addr, uint32_t rank) {
     uint32_t r;

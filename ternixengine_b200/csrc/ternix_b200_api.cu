@@ -289,6 +289,11 @@ int select_kernel(const void* dA, const void* dW, int M, int K, int N) {
 }
 
 // ---------------------------------------------------------------- launches
+// Bytes between the rows of A and the k-rows of W where they are not K and N / 4 (copies made for the TMA unit); 0: as is.
+struct Pitches {
+    long long a = 0, w = 0;
+};
+
 int launch_generic(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N, long long ldc,
                    cudaStream_t st) {
     const int pitch = N / 4;
@@ -349,12 +354,12 @@ GemvPlan plan_gemv(int M, int K, int N) {
     return plan_gemv_with(M, K, N, 0, 0);
 }
 
-template <int MR, int WORDS>
+template <int MR, int WORDS, typename Epi>
 int launch_gemv_t(const CUtensorMap& tmap, const int8_t* dA, int32_t* dC, int M, int K, int N, long long ldc,
-                  const GemvPlan& p, int32_t* d_status, cudaStream_t st) {
-    auto kern = tb200::ternary_gemv_kernel<MR, WORDS>;
+                  const GemvPlan& p, int32_t* d_status, const Epi& epi, cudaStream_t st) {
+    auto kern = tb200::ternary_gemv_kernel<MR, WORDS, Epi>;
     const size_t smem = tb200::gemv_smem_bytes<MR, WORDS>(p.krange);
-    if (const int rc = ensure_smem_attr<tb200::ternary_gemv_kernel<MR, WORDS>>(
+    if (const int rc = ensure_smem_attr<tb200::ternary_gemv_kernel<MR, WORDS, Epi>>(
             tb200::gemv_smem_bytes<MR, WORDS>(tb200::kGemvMaxASlice / MR)))
         return rc;
     const int chunks = (N + WORDS * 16 - 1) / (WORDS * 16);
@@ -371,20 +376,22 @@ int launch_gemv_t(const CUtensorMap& tmap, const int8_t* dA, int32_t* dC, int M,
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const int a_words_ok = (K % 4 == 0) && aligned(dA, 4);
-    TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap, dA, dC, M, K, N, ldc, p.krange, a_words_ok, d_status));
+    TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap, dA, dC, M, K, N, ldc, p.krange, a_words_ok, d_status, epi));
     return TERNIX_B200_OK;
 }
 
+// w_pitch: bytes between the k-rows of W (N / 4 in the packed format; more in a copy made for the TMA unit).
+template <typename Epi = tb200::StoreInt32>
 int launch_gemv(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N, long long ldc,
-                int32_t* d_status, cudaStream_t st) {
+                int32_t* d_status, cudaStream_t st, const Epi& epi = {}, long long w_pitch = 0) {
     const GemvPlan p = plan_gemv(M, K, N);
     if (p.words == 0) return TERNIX_B200_ERR_UNSUPPORTED;
     const int stage_rows = 8 * (32 / p.words) * 4;
     CUtensorMap tmap;
     const int rc = make_tmap_2d(&tmap, dW, static_cast<uint64_t>(N / 4), static_cast<uint64_t>(K),
-                                static_cast<uint64_t>(N / 4), p.words * 4, stage_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
+                                static_cast<uint64_t>(w_pitch ? w_pitch : N / 4), p.words * 4, stage_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (rc) return rc;
-#define TB_GEMV(MR_, W_) launch_gemv_t<MR_, W_>(tmap, dA, dC, M, K, N, ldc, p, d_status, st)
+#define TB_GEMV(MR_, W_) launch_gemv_t<MR_, W_>(tmap, dA, dC, M, K, N, ldc, p, d_status, epi, st)
     if (p.words == 32) {
         if (M == 1) return TB_GEMV(1, 32);
         if (M == 2) return TB_GEMV(2, 32);
@@ -399,13 +406,13 @@ int launch_gemv(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, 
 
 // ---------------------------------------------------------------- batched decode on mma.sync (kernel_decode_mma.cuh)
 int make_mma_problem(tb200::MmaProblem* out, const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N,
-                     long long ldc) {
+                     long long ldc, const Pitches& pt = {}) {
     *out = tb200::MmaProblem{};
     int rc = make_tmap_2d(&out->tmap_w, dW, static_cast<uint64_t>(N / 4), static_cast<uint64_t>(K),
-                          static_cast<uint64_t>(N / 4), tb200::kMmaItemCols / 4, tb200::kMmaStageRows,
+                          static_cast<uint64_t>(pt.w ? pt.w : N / 4), tb200::kMmaItemCols / 4, tb200::kMmaStageRows,
                           CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    rc = make_tmap_2d(&out->tmap_a, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(K), 64,
+    rc = make_tmap_2d(&out->tmap_a, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(pt.a ? pt.a : K), 64,
                       tb200::kMmaBoxRows, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
     out->C = dC;
@@ -417,21 +424,21 @@ int make_mma_problem(tb200::MmaProblem* out, const int8_t* dA, const uint8_t* dW
     return TERNIX_B200_OK;
 }
 
-template <bool kSingle, int NG>
+template <bool kSingle, int NG, typename Epi = tb200::StoreInt32>
 int decode_mma_attr() {
-    return ensure_smem_attr<tb200::ternary_decode_mma_kernel<kSingle, NG>>(tb200::kMmaSmemBytes);
+    return ensure_smem_attr<tb200::ternary_decode_mma_kernel<kSingle, NG, Epi>>(tb200::kMmaSmemBytes);
 }
 
 // One problem: items enumerated in the kernel.  When whole-K items would leave most of the GPU idle the K range is
 // cut into slices that add into a zeroed C.
-template <int NG>
+template <int NG, typename Epi>
 int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N, long long ldc,
-                        int32_t* d_status, cudaStream_t st) {
+                        int32_t* d_status, const Epi& epi, const Pitches& pt, cudaStream_t st) {
     tb200::MmaProblem prob;
-    int rc = make_mma_problem(&prob, dA, dW, dC, M, K, N, ldc);
+    int rc = make_mma_problem(&prob, dA, dW, dC, M, K, N, ldc, pt);
     if (rc) return rc;
-    if ((rc = decode_mma_attr<true, NG>())) return rc;
-    auto kern = tb200::ternary_decode_mma_kernel<true, NG>;
+    if ((rc = decode_mma_attr<true, NG, Epi>())) return rc;
+    auto kern = tb200::ternary_decode_mma_kernel<true, NG, Epi>;
     tb200::MmaSingle sg{};
     sg.group_rows = 8 * NG;
     sg.chunks = (N + tb200::kMmaItemCols - 1) / tb200::kMmaItemCols;
@@ -457,6 +464,7 @@ int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M,
     }
     const Options& o = options();
     if (o.mma_slices > 0) slices = std::max(1, std::min(o.mma_slices, sg.total_tiles));
+    if constexpr (Epi::kFused) slices = 1;         // slices add int32 into C: only whole sums reach the fused epilogue
     // Cluster form: the largest cluster that still leaves one item per resident CTA (option mma_cluster = 0|2|4|8
     // overrides; a forced slice count switches the cluster form off).
     int cluster = 0;
@@ -465,7 +473,7 @@ int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M,
     if (o.mma_cluster >= 0) {
         const int c = o.mma_cluster;
         cluster = ((c == 2 || c == 4 || c == 8) && base_items * c <= resident) ? c : 0;
-    } else if (o.mma_slices > 0) {
+    } else if (o.mma_slices > 0 && !Epi::kFused) {
         cluster = 0;
     }
     if (cluster) {
@@ -488,7 +496,7 @@ int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M,
         const tb200::MmaProblem* no_probs = nullptr;
         const tb200::MmaItem* no_items = nullptr;
         const int* no_first = nullptr;
-        TB_CUDA(cudaLaunchKernelEx(&cfg, kern, prob, sg, no_probs, no_items, no_first, d_status));
+        TB_CUDA(cudaLaunchKernelEx(&cfg, kern, prob, sg, no_probs, no_items, no_first, d_status, epi));
         return TERNIX_B200_OK;
     }
     sg.tiles_per_slice = (sg.total_tiles + slices - 1) / slices;
@@ -496,16 +504,17 @@ int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M,
     sg.add = sg.slices > 1;
     if (sg.add) TB_CUDA(cudaMemset2DAsync(dC, static_cast<size_t>(ldc) * 4, 0, static_cast<size_t>(N) * 4, M, st));
     const int grid = std::min(resident, base_items * sg.slices);
-    kern<<<grid, tb200::kMmaThreads, tb200::kMmaSmemBytes, st>>>(prob, sg, nullptr, nullptr, nullptr, d_status);
+    kern<<<grid, tb200::kMmaThreads, tb200::kMmaSmemBytes, st>>>(prob, sg, nullptr, nullptr, nullptr, d_status, epi);
     TB_CUDA(cudaGetLastError());
     return TERNIX_B200_OK;
 }
 
 // Row groups of 8 up to 8 rows (half the tensor instructions), of 16 beyond.
+template <typename Epi = tb200::StoreInt32>
 int launch_decode_mma(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N, long long ldc,
-                      int32_t* d_status, cudaStream_t st) {
-    if (M <= 8) return launch_decode_mma_t<1>(dA, dW, dC, M, K, N, ldc, d_status, st);
-    return launch_decode_mma_t<2>(dA, dW, dC, M, K, N, ldc, d_status, st);
+                      int32_t* d_status, cudaStream_t st, const Epi& epi = {}, const Pitches& pt = {}) {
+    if (M <= 8) return launch_decode_mma_t<1>(dA, dW, dC, M, K, N, ldc, d_status, epi, pt, st);
+    return launch_decode_mma_t<2>(dA, dW, dC, M, K, N, ldc, d_status, epi, pt, st);
 }
 
 template <int BN>
@@ -588,22 +597,22 @@ int tc3_tile_rows(int M) {
     return M <= 128 ? 128 : 256;
 }
 
-int make_tc3_act_map(CUtensorMap* out, const int8_t* dA, int M, int K, int tile_rows = 256) {
-    return make_tmap_2d(out, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(K), tb200::kTcBK,
+int make_tc3_act_map(CUtensorMap* out, const int8_t* dA, int M, int K, int tile_rows = 256, long long pitch = 0) {
+    return make_tmap_2d(out, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(pitch ? pitch : K), tb200::kTcBK,
                         tile_rows / 2, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-int make_tc3_weight_map(CUtensorMap* out, const uint8_t* dW, int K, int N) {
-    return make_tmap_2d(out, dW, static_cast<uint64_t>(N / 4), static_cast<uint64_t>(K), static_cast<uint64_t>(N / 4),
+int make_tc3_weight_map(CUtensorMap* out, const uint8_t* dW, int K, int N, long long pitch = 0) {
+    return make_tmap_2d(out, dW, static_cast<uint64_t>(N / 4), static_cast<uint64_t>(K), static_cast<uint64_t>(pitch ? pitch : N / 4),
                         tb200::kTc3WpRowBytes, tb200::kTc3BK, CU_TENSOR_MAP_SWIZZLE_32B);
 }
 int make_tc3_store_map(CUtensorMap* out, int32_t* dC, int M, int N, long long ldc) {
     return make_tmap_2d_u32(out, dC, static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(ldc) * 4, 128, 32);
 }
 
-template <int TA>
+template <int TA, typename Epi>
 int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const tb200::Tc3Stores& stores, int32_t* dC0,
-                           int M, int K, int N, long long ldc, int32_t* d_status, cudaStream_t st) {
-    if (const int arc = ensure_smem_attr<tb200::ternary_gemm_tc3_kernel<false, false, TA>>(tb200::tc3_smem_bytes<TA>())) return arc;
+                           int M, int K, int N, long long ldc, int32_t* d_status, const Epi& epi, cudaStream_t st) {
+    if (const int arc = ensure_smem_attr<tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>>(tb200::tc3_smem_bytes<TA>())) return arc;
     const long tiles = static_cast<long>((M + TA - 1) / TA) * ((N + tb200::kTc3TileW - 1) / tb200::kTc3TileW);
     const long max_pairs = sm_count() / 2;
     const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
@@ -622,17 +631,18 @@ int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w,
     const tb200::Tc3Problem* no_probs = nullptr;
     const tb200::Tc2Tile* no_tiles = nullptr;
     const int* no_first = nullptr;
-    TB_CUDA(cudaLaunchKernelEx(&cfg, tb200::ternary_gemm_tc3_kernel<false, false, TA>, tmap_a, tmap_w, stores, dC0, M, K, N, ldc,
-                               no_probs, no_tiles, no_first, d_status, static_cast<const float*>(nullptr), 1.0f));
+    TB_CUDA(cudaLaunchKernelEx(&cfg, tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>, tmap_a, tmap_w, stores, dC0, M, K, N, ldc,
+                               no_probs, no_tiles, no_first, d_status, static_cast<const float*>(nullptr), 1.0f, epi));
     return TERNIX_B200_OK;
 }
 
 // tmap_a must have been made for tc3_tile_rows(M).
+template <typename Epi = tb200::StoreInt32>
 int launch_gemm_tc3_maps(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const tb200::Tc3Stores& stores, int32_t* dC0,
-                         int M, int K, int N, long long ldc, int32_t* d_status, cudaStream_t st) {
+                         int M, int K, int N, long long ldc, int32_t* d_status, cudaStream_t st, const Epi& epi = {}) {
     if (tc3_tile_rows(M) == 128)
-        return launch_gemm_tc3_maps_t<128>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, st);
-    return launch_gemm_tc3_maps_t<256>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, st);
+        return launch_gemm_tc3_maps_t<128>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, epi, st);
+    return launch_gemm_tc3_maps_t<256>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, epi, st);
 }
 
 int launch_gemm_tc3(const int8_t* dA, const uint8_t* dW, int32_t* const* dC_list, int n_dest, int M, int K, int N,
@@ -739,13 +749,13 @@ int next_skinny_epoch() {
 int skinny_rows_class(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
 
 int make_skinny_problem(tb200::SkProblem* out, const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N,
-                        long long ldc) {
+                        long long ldc, int rows_class = 0, const Pitches& pt = {}) {
     *out = tb200::SkProblem{};
     int rc = make_tmap_2d(&out->tmap_w, dW, static_cast<uint64_t>(N / 4), static_cast<uint64_t>(K),
-                          static_cast<uint64_t>(N / 4), tb200::kSkWpRowBytes, tb200::kSkBK, CU_TENSOR_MAP_SWIZZLE_64B);
+                          static_cast<uint64_t>(pt.w ? pt.w : N / 4), tb200::kSkWpRowBytes, tb200::kSkBK, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
-    rc = make_tmap_2d(&out->tmap_a, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(K), 128,
-                      skinny_rows_class(M), CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tmap_2d(&out->tmap_a, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(pt.a ? pt.a : K), 128,
+                      rows_class ? rows_class : skinny_rows_class(M), CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     out->C = dC;
     out->ldc = ldc;
@@ -755,14 +765,14 @@ int make_skinny_problem(tb200::SkProblem* out, const int8_t* dA, const uint8_t* 
     return TERNIX_B200_OK;
 }
 
-template <int NB, bool kGrouped>
+template <int NB, bool kGrouped, typename Epi = tb200::StoreInt32>
 int launch_skinny_t(const tb200::SkProblem& single, const tb200::SkSingle& sg, const tb200::SkProblem* d_probs,
                     const tb200::SkItem* d_items, const int* d_first, int grid, int* d_flags, int epoch,
-                    int32_t* d_status, cudaStream_t st) {
-    if (const int arc = ensure_smem_attr<tb200::ternary_skinny_tc_kernel<NB, kGrouped>>(tb200::SkGeom<NB>::kSmemBytes))
+                    int32_t* d_status, cudaStream_t st, const Epi& epi = {}) {
+    if (const int arc = ensure_smem_attr<tb200::ternary_skinny_tc_kernel<NB, kGrouped, Epi>>(tb200::SkGeom<NB>::kSmemBytes))
         return arc;
-    tb200::ternary_skinny_tc_kernel<NB, kGrouped><<<grid, tb200::SkGeom<NB>::kThreads, tb200::SkGeom<NB>::kSmemBytes, st>>>(
-        single, sg, d_probs, d_items, d_first, d_flags, epoch, d_status);
+    tb200::ternary_skinny_tc_kernel<NB, kGrouped, Epi><<<grid, tb200::SkGeom<NB>::kThreads, tb200::SkGeom<NB>::kSmemBytes, st>>>(
+        single, sg, d_probs, d_items, d_first, d_flags, epoch, d_status, epi);
     TB_CUDA(cudaGetLastError());
     return TERNIX_B200_OK;
 }
@@ -1064,7 +1074,7 @@ int launch_gemm_tc3_group(const ternix_b200_group* g, int32_t* d_status, cudaStr
     tb200::Tc3Stores none{};
     int32_t* no_c = nullptr;
     TB_CUDA(cudaLaunchKernelEx(&cfg, kern, unused, unused, none, no_c, 0, 0, 0, 0LL, g->d_tc3_probs, g->d_tc_tiles,
-                               g->d_tc_first, d_status, static_cast<const float*>(nullptr), 1.0f));
+                               g->d_tc_first, d_status, static_cast<const float*>(nullptr), 1.0f, tb200::StoreInt32{}));
     return TERNIX_B200_OK;
 }
 
@@ -1169,6 +1179,110 @@ int launch_row_quant_dtype(int dtype, const tb200::RowQuantArgs& p, cudaStream_t
     return launch_row_quant<float, MODE>(p, st);
 }
 
+// ---------------------------------------------------------------- the product with the fused epilogue (epilogue.cuh)
+int launch_generic_fused(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const tb200::FusedEpilogue& epi, cudaStream_t st) {
+    dim3 grid((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes, (M + tb200::kGenRows - 1) / tb200::kGenRows);
+    if (grid.y > 65535) return TERNIX_B200_ERR_INVALID_SHAPE;
+    tb200::ternary_generic_fused_kernel<<<grid, tb200::kGenThreads, 0, st>>>(dA, dW, M, K, N, epi);
+    TB_CUDA(cudaGetLastError());
+    return TERNIX_B200_OK;
+}
+
+// The kernels that read through TMA, on operands that it can describe (pitches in `pt`).  kernel: TERNIX_B200_KERNEL_*,
+// not AUTO or GENERIC.
+int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Pitches& pt,
+                     const tb200::FusedEpilogue& epi, int32_t* d_status, cudaStream_t st) {
+    switch (kernel) {
+        case TERNIX_B200_KERNEL_GEMV:
+            g_last_launched = TERNIX_B200_LAUNCHED_GEMV;
+            return launch_gemv(dA, dW, nullptr, M, K, N, N, d_status, st, epi, pt.w);
+        case TERNIX_B200_KERNEL_DECODE_MMA:
+            g_last_launched = TERNIX_B200_LAUNCHED_DECODE_MMA;
+            return launch_decode_mma(dA, dW, nullptr, M, K, N, N, d_status, st, epi, pt);
+        case TERNIX_B200_KERNEL_SKINNY_TC: {
+            // built for 64 and 128 rows (the dispatch never sends it fewer than 33); whole-K items, so no flags
+            g_last_launched = TERNIX_B200_LAUNCHED_SKINNY_TC;
+            const int rows = M <= 64 ? 64 : 128;
+            tb200::SkProblem prob;
+            if (const int rc = make_skinny_problem(&prob, dA, dW, nullptr, M, K, N, N, rows, pt)) return rc;
+            tb200::SkSingle sg{};
+            int grid = 0;
+            plan_skinny(K, N, false, 0, &sg, &grid);
+            if (rows == 64) return launch_skinny_t<64, false>(prob, sg, nullptr, nullptr, nullptr, grid, nullptr, 0, d_status, st, epi);
+            return launch_skinny_t<128, false>(prob, sg, nullptr, nullptr, nullptr, grid, nullptr, 0, d_status, st, epi);
+        }
+        default: {
+            g_last_launched = TERNIX_B200_LAUNCHED_GEMM_TC3;
+            CUtensorMap tmap_a, tmap_w;
+            if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, tc3_tile_rows(M), pt.a)) return rc;
+            if (const int rc = make_tc3_weight_map(&tmap_w, dW, K, N, pt.w)) return rc;
+            return launch_gemm_tc3_maps(tmap_a, tmap_w, tb200::Tc3Stores{}, nullptr, M, K, N, N, d_status, st, epi);
+        }
+    }
+}
+
+// Operands that the TMA unit cannot describe (ragged pitch or unaligned base), product too large for the generic kernel:
+// copy them to pitches of 16 bytes in stream-ordered scratch and run the kernel that the aligned problem would get.
+int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const tb200::FusedEpilogue& epi,
+                              int32_t* d_status, cudaStream_t st) {
+    const long long a_pitch = (K + 15LL) / 16 * 16, w_pitch = (N / 4 + 15LL) / 16 * 16;
+    cudaMemPool_t pool = nullptr;
+    if (const int rc = host_call_pool(&pool)) return rc;
+    // whether an aligned base and aligned pitches suffice for this kernel is what the pretended sizes ask
+    const int Kp = static_cast<int>(a_pitch), Np = static_cast<int>(w_pitch * 4);
+    const int kernel = select_kernel(nullptr, nullptr, M, Kp, Np);
+    const bool copy_a = kernel != TERNIX_B200_KERNEL_GEMV && (K % 16 != 0 || !aligned(dA, 16));
+    const bool copy_w = N % 64 != 0 || !aligned(dW, 16);
+    const size_t a_bytes = copy_a ? static_cast<size_t>(M) * a_pitch : 0, w_bytes = copy_w ? static_cast<size_t>(K) * w_pitch : 0;
+    uint8_t* tmp = nullptr;
+    TB_CUDA(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&tmp), (a_bytes + 255) / 256 * 256 + w_bytes, pool, st));
+    auto copy = [&](const void* src, long long src_pitch, uint8_t* dst, long long pitch, int width, long long rows) {
+        const long long blocks = std::min<long long>((rows * (pitch / 16) + 255) / 256, 8LL * sm_count());
+        tb200::align_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const uint8_t*>(src), src_pitch, dst,
+                                                                                static_cast<int>(pitch), width, rows);
+        return cudaGetLastError();
+    };
+    Pitches pt;
+    const int8_t* a = dA;
+    const uint8_t* w = dW;
+    cudaError_t e = cudaSuccess;
+    if (copy_a) {
+        e = copy(dA, K, tmp, a_pitch, K, M);
+        a = reinterpret_cast<const int8_t*>(tmp);
+        pt.a = a_pitch;
+    }
+    if (copy_w && e == cudaSuccess) {
+        uint8_t* dst = tmp + (a_bytes + 255) / 256 * 256;
+        e = copy(dW, N / 4, dst, w_pitch, N / 4, K);
+        w = dst;
+        pt.w = w_pitch;
+    }
+    const int rc = e != cudaSuccess ? cuda_fail(e) : launch_fused_tma(kernel, a, w, M, K, N, pt, epi, d_status, st);
+    cudaFreeAsync(tmp, st);
+    return rc;
+}
+
+int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, int N, const tb200::FusedEpilogue& epi,
+                 int32_t* d_status, cudaStream_t st) {
+    switch (kernel) {
+        case TERNIX_B200_KERNEL_GEMV: if (!gemv_ok(dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
+        case TERNIX_B200_KERNEL_DECODE_MMA: if (!decode_mma_ok(dA, dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
+        case TERNIX_B200_KERNEL_SKINNY_TC: if (!skinny_ok(dA, dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
+        case TERNIX_B200_KERNEL_GEMM_TC: if (!gemm_tc_ok(dA, dW, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
+        default: break;
+    }
+    if (K == 0) kernel = TERNIX_B200_KERNEL_GENERIC;           // empty sums: only the epilogue is left
+    if (kernel == TERNIX_B200_KERNEL_AUTO) {
+        kernel = select_kernel(dA, dW, M, K, N);
+        if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 &&
+            (static_cast<double>(M) * K * N >= 3e7 || K >= 512))
+            return launch_fused_aligned_copy(dA, dW, M, K, N, epi, d_status, st);
+    }
+    if (kernel != TERNIX_B200_KERNEL_GENERIC) return launch_fused_tma(kernel, dA, dW, M, K, N, Pitches{}, epi, d_status, st);
+    g_last_launched = TERNIX_B200_LAUNCHED_GENERIC;
+    return launch_generic_fused(dA, dW, M, K, N, epi, st);
+}
+
 // y = bf16_rn((float(c) * row_scale[m]) * w_scale), from an int32 C to up to 8 bfloat16 destinations: the
 // unfused form of the dequantising epilogue, for problems the paired-CTA kernel does not take.
 __global__ void dequant_rows_kernel(const int32_t* __restrict__ C, long long ldc, tb200::Tc2Dest dest, long long ldy,
@@ -1226,7 +1340,7 @@ int launch_gemm_tc3_bf16(const int8_t* dA, const uint8_t* dW, void* const* dY_li
     cfg.numAttrs = 1;
     TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap_a, tmap_w, stores, static_cast<int32_t*>(dY_list[0]), M, K, N, ldy,
                                static_cast<const tb200::Tc3Problem*>(nullptr), static_cast<const tb200::Tc2Tile*>(nullptr),
-                               static_cast<const int*>(nullptr), d_status, row_scale, w_scale));
+                               static_cast<const int*>(nullptr), d_status, row_scale, w_scale, tb200::StoreInt32{}));
     return TERNIX_B200_OK;
 }
 
@@ -2076,10 +2190,10 @@ int ternix_b200_group_run(const ternix_b200_group* g, int32_t* d_status, void* s
         const tb200::MmaSingle sg{};
         if (v == 0)
             tb200::ternary_decode_mma_kernel<false, 1><<<mt.grid, tb200::kMmaThreads, tb200::kMmaSmemBytes, st>>>(
-                none, sg, mt.d_probs, mt.d_items, mt.d_first, d_status);
+                none, sg, mt.d_probs, mt.d_items, mt.d_first, d_status, tb200::StoreInt32{});
         else
             tb200::ternary_decode_mma_kernel<false, 2><<<mt.grid, tb200::kMmaThreads, tb200::kMmaSmemBytes, st>>>(
-                none, sg, mt.d_probs, mt.d_items, mt.d_first, d_status);
+                none, sg, mt.d_probs, mt.d_items, mt.d_first, d_status, tb200::StoreInt32{});
         TB_CUDA(cudaGetLastError());
     }
     for (int v = 0; v < 4; ++v) {
@@ -2462,6 +2576,37 @@ int ternix_b200_glu_quantize(const void* dGate, long long ldg, const void* dUp, 
         return TERNIX_B200_ERR_INVALID_ARG;
     const tb200::RowQuantArgs p{dGate, dUp, dWeight, nullptr, dA, d_row_scale, ldg, ldu, 0, M, K, norm ? eps : -1.0f, w_dtype, activation};
     return launch_row_quant_dtype<tb200::kRowGate>(dtype, p, static_cast<cudaStream_t>(stream));
+}
+
+int ternix_b200_matmul_fused(const int8_t* dA, const uint8_t* dW, const ternix_b200_epilogue* ep, void* dY, long long ldy,
+                             int M, int K, int N, int kernel, int32_t* d_status, void* stream) {
+    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!ep || ldy < N || !dtype_ok(ep->out_dtype) || !activation_ok(ep->activation)) return TERNIX_B200_ERR_INVALID_ARG;
+    if (kernel < TERNIX_B200_KERNEL_AUTO || kernel > TERNIX_B200_KERNEL_SKINNY_TC) return TERNIX_B200_ERR_INVALID_ARG;
+    if (ep->bias && (!dtype_ok(ep->bias_dtype) || !aligned(ep->bias, static_cast<uintptr_t>(dtype_bytes(ep->bias_dtype)))))
+        return TERNIX_B200_ERR_INVALID_ARG;
+    if (ep->residual && ep->ldr < N) return TERNIX_B200_ERR_INVALID_ARG;
+    if (M == 0 || N == 0) return TERNIX_B200_OK;
+    const int e = dtype_bytes(ep->out_dtype);
+    if (!dY || !ep->row_scale || (K > 0 && (!dA || !dW))) return TERNIX_B200_ERR_INVALID_ARG;
+    if (!aligned(dY, static_cast<uintptr_t>(e)) || !aligned(ep->residual, static_cast<uintptr_t>(e)) || !aligned(ep->row_scale, 4) ||
+        !aligned(ep->col_scale, 4))
+        return TERNIX_B200_ERR_INVALID_ARG;
+    tb200::FusedEpilogue epi{};
+    epi.row_scale = ep->row_scale;
+    epi.col_scale = ep->col_scale;
+    epi.w_scale = ep->w_scale;
+    epi.bias = ep->bias;
+    epi.bias_dtype = ep->bias_dtype;
+    epi.act = ep->activation;
+    epi.residual = ep->residual;
+    epi.ldr = ep->ldr;
+    epi.out = dY;
+    epi.ldo = ldy;
+    epi.out_dtype = ep->out_dtype;
+    auto vec = [&](const void* p, long long ld) { return aligned(p, static_cast<uintptr_t>(4 * e)) && (M == 1 || ld % 4 == 0); };
+    epi.vec4 = vec(dY, ldy) && (!ep->residual || vec(ep->residual, ep->ldr));
+    return launch_fused(kernel, dA, dW, M, K, N, epi, d_status, static_cast<cudaStream_t>(stream));
 }
 
 int ternix_b200_matmul_dequant(const int8_t* dA, const uint8_t* dW, void* const* dY_list, int n_dest,
