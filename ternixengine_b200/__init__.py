@@ -417,68 +417,65 @@ def matmul_dequant(a, w_packed, row_scale, w_scale: float, out=None, status=None
 
 
 # --------------------------------------------------------------------------- a quantised layer around the product
+# These three run in a decode loop between kernels of a few microseconds, so their host side is kept short: one pass over
+# each operand's type, device, shape and strides, the stream's address without a Stream object, no device guard where the
+# operands' device is current already.
 ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
 
 
-def _dtype_codes():
-    import torch
+class _Runtime:
+    """What the calls below need of torch, looked up once (the package itself imports without it)."""
 
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-class _OnDevice:
-    """Makes a device current for a library call where it is not already, and hands out the address of the current
-    stream of that device."""
-
-    __slots__ = ("_guard", "_device")
-
-    def __init__(self, device):
+    def __init__(self):
         import torch
 
-        self._device = device
-        self._guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        import torch
-
-        if self._guard is not None:
-            self._guard.__enter__()
-        return torch.cuda.current_stream(self._device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+        self.torch = torch
+        self.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        self.f32, self.i8, self.u8, self.bf16 = torch.float32, torch.int8, torch.uint8, torch.bfloat16
+        self.empty, self.Tensor, self.guard = torch.empty, torch.Tensor, torch.cuda.device
+        self.current_device, self.raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _rows(t, name, device, dtype, shape):
-    """Checks a row-major operand with unit column stride and returns (address, row pitch in elements)."""
+_runtime = None
+
+
+def _rt() -> _Runtime:
+    global _runtime
+    if _runtime is None:
+        _runtime = _Runtime()
+    return _runtime
+
+
+def _rows(t, name, dev, dtype, shape) -> int:
+    """Checks a row-major operand with unit column stride and returns its row pitch in elements."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on cuda:{dev}")
+    ld, inner = t.stride()
     M, K = shape
-    if t.device != device or t.dtype != dtype or tuple(t.shape) != shape or (K > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be {shape} {dtype} on {device} with unit column stride")
-    ld = t.stride(0) if M > 1 else K
+    if inner != 1 and K > 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if M <= 1:
+        return K
     if ld < K:
         raise ValueError(f"{name}: its rows overlap")
-    return t.data_ptr(), ld
+    return ld
 
 
-def _flat(t, name, device, dtypes, n):
-    if t.device != device or t.dtype not in dtypes or tuple(t.shape) != (n,) or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be ({n},) of {' or '.join(str(d) for d in dtypes)} on {device}, contiguous")
+def _vector(t, name, dev, dtypes, n) -> int:
+    """Checks a contiguous vector and returns its address."""
+    if t.dtype not in dtypes or t.get_device() != dev or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be ({n},) of {' or '.join(str(d) for d in dtypes)} on cuda:{dev}, contiguous")
     return t.data_ptr()
 
 
-def _quantized_out(x, out, row_scale):
-    import torch
-
-    M, K = x.shape
+def _quantized_out(rt, dev, shape, out, row_scale):
     if out is None:
-        out = torch.empty((M, K), dtype=torch.int8, device=x.device)
-    elif out.device != x.device or out.dtype != torch.int8 or tuple(out.shape) != (M, K) or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous ({M}, {K}) int8 tensor on {x.device}")
+        out = rt.empty(shape, dtype=rt.i8, device=f"cuda:{dev}")
+    elif out.dtype is not rt.i8 or out.get_device() != dev or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {tuple(shape)} int8 tensor on cuda:{dev}")
     if row_scale is None:
-        row_scale = torch.empty((M,), dtype=torch.float32, device=x.device)
-    _flat(row_scale, "row_scale", x.device, (torch.float32,), M)
-    return out, row_scale
+        row_scale = rt.empty(shape[0], dtype=rt.f32, device=f"cuda:{dev}")
+    return out, row_scale, _vector(row_scale, "row_scale", dev, (rt.f32,), shape[0])
 
 
 def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None, row_scale=None, residual_out=None):
@@ -489,59 +486,70 @@ def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None,
     type or float32, or None.  Returns (codes, row_scale), and h as a third where a residual is given; residual_out may be
     `residual` or `x` itself.  codes x row_scale stands for y: codes = rint(h * weight * 127 / max|h * weight|).  A row of
     zeros has codes 0 and scale 1, a row with an infinity or NaN has codes 0 and scale NaN."""
-    import torch
-
-    codes = _dtype_codes()
-    if not x.is_cuda or x.dim() != 2 or x.dtype not in codes:
+    rt = _rt()
+    dtype = x.dtype
+    code, dev, shape = rt.codes.get(dtype), x.get_device(), x.shape
+    if code is None or dev < 0 or len(shape) != 2:
         raise ValueError("rmsnorm_quantize takes a CUDA (M, K) bfloat16, float16 or float32 tensor")
-    M, K = x.shape
-    px, ldx = _rows(x, "x", x.device, x.dtype, (M, K))
+    ldx = _rows(x, "x", dev, dtype, shape)
+    M, K = shape
     pr = ph = pw = None
     ldr = ldh = w_dtype = 0
     if weight is not None:
-        pw, w_dtype = _flat(weight, "weight", x.device, (x.dtype, torch.float32), K), codes.get(weight.dtype)
-    out, row_scale = _quantized_out(x, out, row_scale)
+        pw, w_dtype = _vector(weight, "weight", dev, (dtype, rt.f32), K), rt.codes[weight.dtype]
+    out, row_scale, ps = _quantized_out(rt, dev, shape, out, row_scale)
     if residual is not None:
-        pr, ldr = _rows(residual, "residual", x.device, x.dtype, (M, K))
+        pr, ldr = residual.data_ptr(), _rows(residual, "residual", dev, dtype, shape)
         if residual_out is None:
-            residual_out = torch.empty((M, K), dtype=x.dtype, device=x.device)
-        ph, ldh = _rows(residual_out, "residual_out", x.device, x.dtype, (M, K))
+            residual_out = rt.empty(shape, dtype=dtype, device=x.device)
+        ph, ldh = residual_out.data_ptr(), _rows(residual_out, "residual_out", dev, dtype, shape)
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
-    with _OnDevice(x.device) as s:
-        _check(lib.ternix_b200_rmsnorm_quantize(px, ldx, pr, ldr, codes[x.dtype], pw, w_dtype, eps, ph, ldh, out.data_ptr(),
-                                                row_scale.data_ptr(), M, K, s), "rmsnorm_quantize")
+    args = (x.data_ptr(), ldx, pr, ldr, code, pw, w_dtype, eps, ph, ldh, out.data_ptr(), ps, M, K, rt.raw_stream(dev))
+    if rt.current_device() == dev:
+        rc = lib.ternix_b200_rmsnorm_quantize(*args)
+    else:
+        with rt.guard(dev):
+            rc = lib.ternix_b200_rmsnorm_quantize(*args)
+    if rc:
+        _check(rc, "rmsnorm_quantize")
     return (out, row_scale) if residual is None else (out, row_scale, residual_out)
 
 
 def glu_quantize(gate, up, activation: str = "silu", weight=None, eps=None, out=None, row_scale=None):
     """The step between a gated feed-forward block's two products: z = act(gate) * up as int8 codes with one float32 scale
-    per row, in one pass on the current stream (ternix_b200_glu_quantize).  With `eps` the row is normalised first, z / rms(z) * weight.
+    per row, in one pass on the current stream (ternix_b200_glu_quantize).  With `eps` the row is normalised first,
+    z / rms(z) * weight.
 
     gate, up: CUDA (M, K) of one type (bfloat16, float16 or float32), unit column stride, any row pitch, e.g. the two halves
     of one product's output.  activation: "none", "relu", "relu2", "silu", "gelu" or "gelu_tanh".  weight: (K,) of the same
     type or float32, only with eps.  Returns (codes, row_scale); rows of zeros and rows with an infinity or NaN as in
     rmsnorm_quantize()."""
-    import torch
-
-    codes = _dtype_codes()
-    if not gate.is_cuda or gate.dim() != 2 or gate.dtype not in codes:
+    rt = _rt()
+    dtype = gate.dtype
+    code, dev, shape = rt.codes.get(dtype), gate.get_device(), gate.shape
+    if code is None or dev < 0 or len(shape) != 2:
         raise ValueError("glu_quantize takes CUDA (M, K) bfloat16, float16 or float32 tensors")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
     if weight is not None and eps is None:
         raise ValueError("a weight belongs to the norm: give eps too")
-    M, K = gate.shape
-    pg, ldg = _rows(gate, "gate", gate.device, gate.dtype, (M, K))
-    pu, ldu = _rows(up, "up", gate.device, gate.dtype, (M, K))
+    ldg, ldu = _rows(gate, "gate", dev, dtype, shape), _rows(up, "up", dev, dtype, shape)
+    M, K = shape
     pw, w_dtype = None, 0
     if weight is not None:
-        pw, w_dtype = _flat(weight, "weight", gate.device, (gate.dtype, torch.float32), K), codes.get(weight.dtype)
-    out, row_scale = _quantized_out(gate, out, row_scale)
-    with _OnDevice(gate.device) as s:
-        _check(lib.ternix_b200_glu_quantize(pg, ldg, pu, ldu, codes[gate.dtype], ACTIVATIONS[activation], eps is not None, pw,
-                                            w_dtype, 0.0 if eps is None else eps, out.data_ptr(), row_scale.data_ptr(), M, K, s),
-               "glu_quantize")
+        pw, w_dtype = _vector(weight, "weight", dev, (dtype, rt.f32), K), rt.codes[weight.dtype]
+    out, row_scale, ps = _quantized_out(rt, dev, shape, out, row_scale)
+    args = (gate.data_ptr(), ldg, up.data_ptr(), ldu, code, act, eps is not None, pw, w_dtype, eps or 0.0, out.data_ptr(), ps, M, K,
+            rt.raw_stream(dev))
+    if rt.current_device() == dev:
+        rc = lib.ternix_b200_glu_quantize(*args)
+    else:
+        with rt.guard(dev):
+            rc = lib.ternix_b200_glu_quantize(*args)
+    if rc:
+        _check(rc, "glu_quantize")
     return out, row_scale
 
 
@@ -555,45 +563,52 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
     "relu2", "silu", "gelu" or "gelu_tanh".  residual: (M, N) of the output's type, unit column stride, any row pitch; may be
     `out` itself.  out: (M, N) bfloat16, float16 or float32, unit column stride, any row pitch; without it a new tensor of
     out_dtype (the residual's type, else bfloat16)."""
-    import torch
-
-    codes = _dtype_codes()
-    if not (a.is_cuda and w_packed.is_cuda):
-        raise ValueError("matmul_fused() takes CUDA tensors")
-    if a.dtype != torch.int8 or w_packed.dtype != torch.uint8 or a.dim() != 2 or w_packed.dim() != 2:
+    rt = _rt()
+    dev, sa, sw = a.get_device(), a.shape, w_packed.shape
+    if dev < 0 or w_packed.get_device() != dev:
+        raise ValueError("matmul_fused() takes CUDA tensors on one device")
+    if a.dtype is not rt.i8 or w_packed.dtype is not rt.u8 or len(sa) != 2 or len(sw) != 2:
         raise ValueError("A must be (M, K) int8 and W_packed (K, N/4) uint8")
-    if w_packed.device != a.device:
-        raise ValueError("A and W_packed must be on one device")
     if not (a.is_contiguous() and w_packed.is_contiguous()):
         raise ValueError("A and W_packed must be contiguous")
-    M, K = a.shape
-    if w_packed.shape[0] != K:
+    M, K = sa
+    if sw[0] != K:
         raise ValueError("inner dimensions do not match")
-    N = w_packed.shape[1] * 4
-    if activation not in ACTIVATIONS:
+    N = sw[1] * 4
+    act, kern = ACTIVATIONS.get(activation), KERNELS.get(kernel)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
-    if kernel not in KERNELS:
+    if kern is None:
         raise ValueError(f"kernel must be one of {', '.join(KERNELS)}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or (torch.bfloat16 if residual is None else residual.dtype), device=a.device)
+        out = rt.empty((M, N), dtype=out_dtype or (rt.bf16 if residual is None else residual.dtype), device=a.device)
     elif out_dtype is not None and out_dtype != out.dtype:
         raise ValueError("out has another type than out_dtype")
-    if out.dtype not in codes:
+    dtype = out.dtype
+    code = rt.codes.get(dtype)
+    if code is None:
         raise ValueError("the output is bfloat16, float16 or float32")
-    py, ldy = _rows(out, "out", a.device, out.dtype, (M, N))
-    ep = _Epilogue(row_scale=_flat(row_scale, "row_scale", a.device, (torch.float32,), M), activation=ACTIVATIONS[activation],
-                   out_dtype=codes[out.dtype])
-    if isinstance(w_scale, torch.Tensor):
-        ep.col_scale = _flat(w_scale, "w_scale", a.device, (torch.float32,), N)
+    ldy = _rows(out, "out", dev, dtype, (M, N))
+    pc = pb = pr = None
+    ws, b_dtype, ldr = 0.0, 0, 0
+    if isinstance(w_scale, rt.Tensor):
+        pc = _vector(w_scale, "w_scale", dev, (rt.f32,), N)
     else:
-        ep.w_scale = w_scale
+        ws = w_scale
     if bias is not None:
-        ep.bias, ep.bias_dtype = _flat(bias, "bias", a.device, codes, N), codes.get(bias.dtype, 0)
+        pb, b_dtype = _vector(bias, "bias", dev, rt.codes, N), rt.codes[bias.dtype]
     if residual is not None:
-        ep.residual, ep.ldr = _rows(residual, "residual", a.device, out.dtype, (M, N))
-    with _OnDevice(a.device) as s:
-        _check(lib.ternix_b200_matmul_fused(a.data_ptr(), w_packed.data_ptr(), ctypes.byref(ep), py, ldy, M, K, N, KERNELS[kernel],
-                                            status.data_ptr() if status is not None else None, s), "matmul_fused")
+        pr, ldr = residual.data_ptr(), _rows(residual, "residual", dev, dtype, (M, N))
+    ep = _Epilogue(_vector(row_scale, "row_scale", dev, (rt.f32,), M), pc, ws, act, pb, b_dtype, code, pr, ldr)
+    args = (a.data_ptr(), w_packed.data_ptr(), ep, out.data_ptr(), ldy, M, K, N, kern,
+            status.data_ptr() if status is not None else None, rt.raw_stream(dev))
+    if rt.current_device() == dev:
+        rc = lib.ternix_b200_matmul_fused(*args)
+    else:
+        with rt.guard(dev):
+            rc = lib.ternix_b200_matmul_fused(*args)
+    if rc:
+        _check(rc, "matmul_fused")
     return out
 
 

@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 namespace tb200 {
 
@@ -32,22 +33,53 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// One instruction each: maximum that keeps a NaN, 2^x (relative error 2^-22) and 1 / x (1 ulp), subnormals flushed.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// v / (1 + exp(-u)).  The exponential's error, 2^-22 and |u| 2^-23 from its argument, is weighed by exp(-u) / (1 + exp(-u));
+// a denominator above 2^126 gives 0 (the quotient is below |v| 2^-126).
+__device__ __forceinline__ float logistic_times(float v, float u) {
+    return v * rcp_approx(1.0f + exp2_approx(-1.44269504f * u));
+}
+// v (1 + erf(v / sqrt 2)) / 2 through erfc: Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26,
+//   erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) + e,  t = 1 / (1 + p x),  x >= 0,  |e| <= 1.5e-7,
+// which is what fp32 resolves next to 1; a third of the instructions of the library's erf.
+__device__ __forceinline__ float gelu(float v) {
+    const float x = fabsf(v) * 0.70710678f;
+    const float t = rcp_approx(fmaf(0.3275911f, x, 1.0f));
+    float s = fmaf(1.061405429f, t, -1.453152027f);
+    s = fmaf(s, t, 1.421413741f);
+    s = fmaf(s, t, -0.284496736f);
+    s = fmaf(s, t, 0.254829592f);
+    const float half_erfc = 0.5f * (s * t) * exp2_approx(-1.44269504f * (x * x));
+    return v * (v < 0.0f ? half_erfc : 1.0f - half_erfc);
+}
 // act(v) on N values at once: the choice is the same for the whole launch, so it is made once per N values.  A NaN stays
-// a NaN in every activation.  The logistic function is v / (1 + exp(-v)) on the hardware's exponential: its error, a
-// few units in the 24th bit for arguments that matter, is weighed by v * exp(-v) for positive v and by the result's own
-// smallness for negative v, and stays under 3e-7 of the result's scale.
-__device__ __forceinline__ float logistic_times(float v, float u) { return __fdividef(v, 1.0f + __expf(-u)); }
+// a NaN in every activation.
 template <int N>
 __device__ __forceinline__ void activate(int act, float (&v)[N]) {
     switch (act) {
         case kActRelu:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+            for (int i = 0; i < N; ++i) v[i] = max_nan(v[i], 0.0f);
             break;
         case kActRelu2:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float r = v[i] < 0.0f ? 0.0f : v[i];
+                const float r = max_nan(v[i], 0.0f);
                 v[i] = __fmul_rn(r, r);
             }
             break;
@@ -57,7 +89,7 @@ __device__ __forceinline__ void activate(int act, float (&v)[N]) {
             break;
         case kActGelu:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
+            for (int i = 0; i < N; ++i) v[i] = gelu(v[i]);
             break;
         case kActGeluTanh:       // 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
 #pragma unroll
@@ -73,8 +105,11 @@ struct StoreInt32 {
     static constexpr bool kFused = false;
 };
 
+// k32: the output and the residual are float32; else 16 bits wide, bfloat16 or float16 by out_dtype.
+template <bool k32>
 struct FusedEpilogue {
     static constexpr bool kFused = true;
+    using Raw = std::conditional_t<k32, uint4, uint2>;       // four residual values as they lie in memory
     const float* row_scale;        // [M]
     const float* col_scale;        // [N], or null: w_scale for every column
     const void* bias;              // [N] of bias_dtype, or null
@@ -92,22 +127,27 @@ struct FusedEpilogue {
         if (bias_dtype == kDtypeBf16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(bias) + col));
         return __half2float(__ldg(static_cast<const __half*>(bias) + col));
     }
-    // Before the activation.  Without a bias nothing is added (0 would turn -0 into +0: harmless, and one instruction).
+    // Before the activation.  Without a bias 0 is added, which only turns -0 into +0.
     __device__ __forceinline__ float linear(int32_t c, float rs, float cs, float b) const {
         return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(c), rs), cs), b);
     }
 
-    template <typename T>
-    __device__ __forceinline__ void finish_t(int row, int col, float v) const {
-        T* o = static_cast<T*>(out) + static_cast<size_t>(row) * ldo + col;
-        if (residual) v = __fadd_rn(v, to_float<T>(static_cast<const T*>(residual)[static_cast<size_t>(row) * ldr + col]));
-        *o = from_float<T>(v);
+    __device__ __forceinline__ float from_bits(uint32_t b) const {           // low 16 bits
+        return out_dtype == kDtypeBf16 ? __uint_as_float(b << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(b)));
+    }
+    __device__ __forceinline__ uint32_t to_bits(float v) const {
+        return out_dtype == kDtypeBf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
     }
     // One activated value: residual and store.
     __device__ __forceinline__ void finish(int row, int col, float v) const {
-        if (out_dtype == kDtypeBf16) finish_t<__nv_bfloat16>(row, col, v);
-        else if (out_dtype == kDtypeF16) finish_t<__half>(row, col, v);
-        else finish_t<float>(row, col, v);
+        const size_t at_r = static_cast<size_t>(row) * ldr + col, at_o = static_cast<size_t>(row) * ldo + col;
+        if constexpr (k32) {
+            if (residual) v = __fadd_rn(v, static_cast<const float*>(residual)[at_r]);
+            static_cast<float*>(out)[at_o] = v;
+        } else {
+            if (residual) v = __fadd_rn(v, from_bits(static_cast<const uint16_t*>(residual)[at_r]));
+            static_cast<uint16_t*>(out)[at_o] = static_cast<uint16_t>(to_bits(v));
+        }
     }
     __device__ __forceinline__ void store(int row, int col, int32_t c) const {
         float v[1] = {linear(c, __ldg(row_scale + row), column_scale(col), column_bias(col))};
@@ -115,54 +155,62 @@ struct FusedEpilogue {
         finish(row, col, v[0]);
     }
 
-    // The residual of four columns, as it lies in memory (vec4 only): issued early, used by finish4().
-    __device__ __forceinline__ uint4 load_residual4(int row, int col) const {
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (!residual || !vec4) return raw;
+    // The residual of columns col .. col + 3 (col a multiple of four): issued early, used by finish4().
+    __device__ __forceinline__ Raw load_residual4(int row, int col) const {
+        Raw raw{};
+        if (!residual) return raw;
         const size_t at = static_cast<size_t>(row) * ldr + col;
-        if (out_dtype == kDtypeF32) {
-            raw = *reinterpret_cast<const uint4*>(static_cast<const float*>(residual) + at);
+        if constexpr (k32) {
+            const float* p = static_cast<const float*>(residual) + at;
+            if (vec4) raw = *reinterpret_cast<const uint4*>(p);
+            else raw = make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3]));
         } else {
-            const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(residual) + at);
-            raw.x = r.x;
-            raw.y = r.y;
+            const uint16_t* p = static_cast<const uint16_t*>(residual) + at;
+            if (vec4) raw = *reinterpret_cast<const uint2*>(p);
+            else raw = make_uint2(p[0] | static_cast<uint32_t>(p[1]) << 16, p[2] | static_cast<uint32_t>(p[3]) << 16);
         }
         return raw;
     }
-    template <typename T>
-    __device__ __forceinline__ void finish4_half(int row, int col, float (&v)[4], const uint4& raw) const {
-        union { uint2 u; T t[4]; } x;
-        if (residual) {
-            x.u = make_uint2(raw.x, raw.y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(v[i], to_float<T>(x.t[i]));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.t[i] = from_float<T>(v[i]);
-        *reinterpret_cast<uint2*>(static_cast<T*>(out) + static_cast<size_t>(row) * ldo + col) = x.u;
+    // Asks for `count` residual values of a row to be brought into L2.
+    __device__ __forceinline__ void prefetch_residual(int row, int col, int count) const {
+        constexpr int kBytes = k32 ? 4 : 2;
+        const char* p = static_cast<const char*>(residual) + (static_cast<size_t>(row) * ldr + col) * kBytes;
+        for (int b = 0; b < count * kBytes; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + b));
     }
-    // Four activated values of columns col .. col + 3 (col a multiple of four).
-    __device__ __forceinline__ void finish4(int row, int col, float (&v)[4], const uint4& raw) const {
-        if (!vec4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) finish(row, col + i, v[i]);
-        } else if (out_dtype == kDtypeBf16) {
-            finish4_half<__nv_bfloat16>(row, col, v, raw);
-        } else if (out_dtype == kDtypeF16) {
-            finish4_half<__half>(row, col, v, raw);
+    // Four activated values of columns col .. col + 3.
+    __device__ __forceinline__ void finish4(int row, int col, const float* v, const Raw& raw) const {
+        const size_t at = static_cast<size_t>(row) * ldo + col;
+        if constexpr (k32) {
+            float4 y = make_float4(v[0], v[1], v[2], v[3]);
+            if (residual)
+                y = make_float4(__fadd_rn(y.x, __uint_as_float(raw.x)), __fadd_rn(y.y, __uint_as_float(raw.y)),
+                                __fadd_rn(y.z, __uint_as_float(raw.z)), __fadd_rn(y.w, __uint_as_float(raw.w)));
+            float* o = static_cast<float*>(out) + at;
+            if (vec4) *reinterpret_cast<float4*>(o) = y;
+            else { o[0] = y.x; o[1] = y.y; o[2] = y.z; o[3] = y.w; }
         } else {
+            float y[4] = {v[0], v[1], v[2], v[3]};
             if (residual) {
-                v[0] = __fadd_rn(v[0], __uint_as_float(raw.x));
-                v[1] = __fadd_rn(v[1], __uint_as_float(raw.y));
-                v[2] = __fadd_rn(v[2], __uint_as_float(raw.z));
-                v[3] = __fadd_rn(v[3], __uint_as_float(raw.w));
+                y[0] = __fadd_rn(y[0], from_bits(raw.x & 0xffffu));
+                y[1] = __fadd_rn(y[1], from_bits(raw.x >> 16));
+                y[2] = __fadd_rn(y[2], from_bits(raw.y & 0xffffu));
+                y[3] = __fadd_rn(y[3], from_bits(raw.y >> 16));
             }
-            *reinterpret_cast<float4*>(static_cast<float*>(out) + static_cast<size_t>(row) * ldo + col) =
-                make_float4(v[0], v[1], v[2], v[3]);
+            uint32_t lo, hi;             // two roundings and the packing are one instruction
+            if (out_dtype == kDtypeBf16) {
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(y[1]), "f"(y[0]));
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y[3]), "f"(y[2]));
+            } else {
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(y[1]), "f"(y[0]));
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y[3]), "f"(y[2]));
+            }
+            uint16_t* o = static_cast<uint16_t*>(out) + at;
+            if (vec4) *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
+            else { o[0] = lo & 0xffffu; o[1] = lo >> 16; o[2] = hi & 0xffffu; o[3] = hi >> 16; }
         }
     }
     __device__ __forceinline__ void store4(int row, int col, const int32_t (&c)[4]) const {
-        const uint4 raw = load_residual4(row, col);
+        const Raw raw = load_residual4(row, col);
         const float rs = __ldg(row_scale + row);
         float v[4];
 #pragma unroll

@@ -151,9 +151,8 @@ __device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
-// ... and in both CTAs of the pair (CTA mask 0b11).
-__device__ __forceinline__ void tc_commit_pair_both(uint64_t* bar) {
-    const uint16_t mask = 3;
+// ... and in both CTAs of the pair (`mask`: their bits among the cluster's CTAs).
+__device__ __forceinline__ void tc_commit_pair_both(uint64_t* bar, uint16_t mask = 3) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::
                      "r"(smem_u32(bar)), "h"(mask)
                  : "memory");

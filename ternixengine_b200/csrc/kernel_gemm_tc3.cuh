@@ -543,6 +543,12 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             const long long ldc = w.ldc;
             int32_t* C = w.C;
             const uint32_t ab = lt % BUFS;
+            if constexpr (Epi::kFused) {
+                // the tile's residual into L2 while its MMAs run: one row of it per thread
+                const int row = a_t * TA + static_cast<int>((warp - kTc3FirstEpilogueWarp) * 32 + lane);
+                const int col = w.w_t * kTc3TileW + rank * 128;
+                if (epi.residual && row < M && row < (a_t + 1) * TA && col < N) epi.prefetch_residual(row, col, min(128, N - col));
+            }
             if (!mbar_wait_backoff(&acc_full[ab], (lt / BUFS) & 1, abort_flag, TB200_TC3_ACC_SLEEP_NS)) { ok = false; break; }
             tc_fence_after_sync();
             const int col0 = w.w_t * kTc3TileW + rank * 128;
@@ -570,24 +576,47 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         sts_u32(buf + ((j * 128 + colp) << 2), static_cast<uint32_t>(static_cast<int32_t>(r[i][j]) >> 6));
-                    asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
-                    const int col = col0 + 4 * lane;
-                    if (col < N) {
-                        float cs[4], b[4];
+                    // Everything the step needs from global memory is requested here, before the barrier, so that its
+                    // latency is met once per step: the residual of this warp's eight rows (four at a time in float32),
+                    // their scales (lane j holds row j's) and, for the tile, the columns' scales and biases.
+                    const int col = col0 + 4 * lane, first = row0 + 8 * static_cast<int>(q);
+                    constexpr int kAhead = sizeof(typename Epi::Raw) == 8 ? 8 : 4;
+                    typename Epi::Raw raw[kAhead];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) { cs[x] = epi.column_scale(col + x); b[x] = epi.column_bias(col + x); }
-                        const int first = row0 + 8 * static_cast<int>(q), rows = min(8, M - first);
-#pragma unroll 2
-                        for (int j = 0; j < rows; ++j) {
-                            const uint4 raw = epi.load_residual4(first + j, col);
-                            const uint4 sum = lds_v4(buf + ((8 * q + j) * 128 + 4 * lane) * 4);
-                            const float rs = __ldg(epi.row_scale + first + j);
-                            float v[4] = {epi.linear(static_cast<int32_t>(sum.x), rs, cs[0], b[0]),
-                                          epi.linear(static_cast<int32_t>(sum.y), rs, cs[1], b[1]),
-                                          epi.linear(static_cast<int32_t>(sum.z), rs, cs[2], b[2]),
-                                          epi.linear(static_cast<int32_t>(sum.w), rs, cs[3], b[3])};
-                            activate(epi.act, v);
-                            epi.finish4(first + j, col, v, raw);
+                    for (int j = 0; j < kAhead; ++j) {
+                        raw[j] = typename Epi::Raw{};
+                        if (col < N && first + j < M) raw[j] = epi.load_residual4(first + j, col);
+                    }
+                    const float rs_lane = first + (lane & 7) < M ? __ldg(epi.row_scale + first + (lane & 7)) : 0.0f;
+                    float cs[4], b[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        cs[x] = col < N ? epi.column_scale(col + x) : 0.0f;
+                        b[x] = col < N ? epi.column_bias(col + x) : 0.0f;
+                    }
+                    asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[16];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint4 sum = lds_v4(buf + ((8 * q + 4 * h + j) * 128 + 4 * lane) * 4);
+                            const float rs = __shfl_sync(0xffffffffu, rs_lane, 4 * h + j);
+                            v[4 * j] = epi.linear(static_cast<int32_t>(sum.x), rs, cs[0], b[0]);
+                            v[4 * j + 1] = epi.linear(static_cast<int32_t>(sum.y), rs, cs[1], b[1]);
+                            v[4 * j + 2] = epi.linear(static_cast<int32_t>(sum.z), rs, cs[2], b[2]);
+                            v[4 * j + 3] = epi.linear(static_cast<int32_t>(sum.w), rs, cs[3], b[3]);
+                        }
+                        activate(epi.act, v);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (col < N && first + 4 * h + j < M) epi.finish4(first + 4 * h + j, col, v + 4 * j, raw[(4 * h + j) % kAhead]);
+                        if constexpr (kAhead == 4) {
+                            if (h == 0) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    if (col < N && first + 4 + j < M) raw[j] = epi.load_residual4(first + 4 + j, col);
+                            }
                         }
                     }
                     __syncwarp();

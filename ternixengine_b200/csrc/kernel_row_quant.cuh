@@ -93,11 +93,6 @@ __device__ __forceinline__ void row_element(const RowQuantArgs& p, int row, int 
         for (int i = 0; i < V; ++i) v[i] = __fmul_rn(v[i], to_float<T>(y.t[i]));
     }
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 // Codes as the low bytes of t * inv + 1.5 * 2^23: the addition rounds to the nearest integer, ties to even, and leaves
 // it in two's complement in the low bits; |t * inv| <= 127 (1 + 2^-22).
 __device__ __forceinline__ uint32_t row_code(float t, float inv) {

@@ -540,16 +540,19 @@ ternary_skinny_tc_kernel(const __grid_constant__ SkProblem single, const SkSingl
                         const float cs = col < N ? epi.column_scale(col) : 0.0f, b = col < N ? epi.column_bias(col) : 0.0f;
 #pragma unroll
                         for (int c = 0; c < kBatch; ++c) {
-                            float v[16];
+                            const int first = 16 * (c0 + c);
+                            const float rs_lane = first + (lane & 15) < M ? __ldg(epi.row_scale + first + (lane & 15)) : 0.0f;
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const int row = 16 * (c0 + c) + j;
-                                v[j] = epi.linear(static_cast<int32_t>(r[c][j]) >> 6, row < M ? __ldg(epi.row_scale + row) : 0.0f, cs, b);
+                            for (int g = 0; g < 16; g += 8) {
+                                float v[8];
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    v[j] = epi.linear(static_cast<int32_t>(r[c][g + j]) >> 6, __shfl_sync(0xffffffffu, rs_lane, g + j), cs, b);
+                                activate(epi.act, v);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    if (first + g + j < M && col < N) epi.finish(first + g + j, col, v[j]);
                             }
-                            activate(epi.act, v);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                if (16 * (c0 + c) + j < M && col < N) epi.finish(16 * (c0 + c) + j, col, v[j]);
                         }
                         __syncwarp();          // the tensor-memory instructions of the next batch want the warp together
                         continue;

@@ -19,6 +19,7 @@
 
 #include "kernel_gemm_tc.cuh"
 #include "kernel_gemm_tc2.cuh"
+#include "kernel_gemm_split.cuh"
 #include "kernel_gemm_tc3.cuh"
 #include "kernel_gemv.cuh"
 #include "kernel_decode_mma.cuh"
@@ -165,6 +166,7 @@ struct Options {
     int skinny_lo = 33, skinny_hi = 64; // rows of a single product served by the tensor-memory decode kernel (0,0 = never)
     int skinny_group_lo = 17, skinny_group_hi = 128;   // the same for members of a problem group (one launch serves many products there)
     int skinny_split = 1;              // 0: never share a block between CTAs; 1: only when blocks outnumber SMs; 2: whenever it evens the load
+    int split_rows = 0, split_cut = 0; // fused product: tile rows (64|128|256) and pairs per tile (1|2|4) of the cut prefill form; 0 = by shape
     int host_slab = -1;                // slab extent of the pipelined host-pointer call; 0 = off, -1 = plan
     bool host_slab_rows = false;
 };
@@ -197,6 +199,9 @@ int apply_option(const char* name, const char* value) {
         g_opt.skinny_group_lo = def.skinny_group_lo; g_opt.skinny_group_hi = def.skinny_group_hi;
         if (!reset && std::sscanf(value, "%d,%d", &g_opt.skinny_group_lo, &g_opt.skinny_group_hi) == 1)
             g_opt.skinny_group_hi = def.skinny_group_hi;
+    } else if (!std::strcmp(name, "fused_split")) {
+        g_opt.split_rows = def.split_rows; g_opt.split_cut = def.split_cut;
+        if (!reset) std::sscanf(value, "%d,%d", &g_opt.split_rows, &g_opt.split_cut);
     } else if (!std::strcmp(name, "host_slab")) {
         g_opt.host_slab = def.host_slab; g_opt.host_slab_rows = false;
         if (!reset) {
@@ -211,7 +216,7 @@ const Options& options() {
     static std::once_flag once;
     std::call_once(once, [] {
         static const char* const names[] = {"tc3", "tc_tile_rows", "tc_bn", "tc_ksplit", "gemv_plan", "group_words", "gemv_pdl", "mma_rows", "mma_slices",
-                                            "mma_cluster", "skinny_rows", "skinny_group_rows", "skinny_split", "host_slab"};
+                                            "mma_cluster", "skinny_rows", "skinny_group_rows", "skinny_split", "fused_split", "host_slab"};
         std::lock_guard<std::mutex> lock(g_opt_mutex);
         for (const char* n : names) {
             char env[64] = "TERNIX_B200_";
@@ -1180,7 +1185,8 @@ int launch_row_quant_dtype(int dtype, const tb200::RowQuantArgs& p, cudaStream_t
 }
 
 // ---------------------------------------------------------------- the product with the fused epilogue (epilogue.cuh)
-int launch_generic_fused(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const tb200::FusedEpilogue& epi, cudaStream_t st) {
+template <typename Epi>
+int launch_generic_fused(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Epi& epi, cudaStream_t st) {
     dim3 grid((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes, (M + tb200::kGenRows - 1) / tb200::kGenRows);
     if (grid.y > 65535) return TERNIX_B200_ERR_INVALID_SHAPE;
     tb200::ternary_generic_fused_kernel<<<grid, tb200::kGenThreads, 0, st>>>(dA, dW, M, K, N, epi);
@@ -1188,10 +1194,47 @@ int launch_generic_fused(const int8_t* dA, const uint8_t* dW, int M, int K, int 
     return TERNIX_B200_OK;
 }
 
+// The cut prefill form (kernel_gemm_split.cuh): tile rows, and pairs that share a tile's K.
+template <int TA, typename Epi>
+int launch_gemm_split_t(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Pitches& pt, int cut, const Epi& epi,
+                        int32_t* d_status, cudaStream_t st) {
+    constexpr auto kern = tb200::ternary_gemm_split_kernel<TA, Epi>;
+    if (const int rc = ensure_smem_attr<kern>(tb200::SpGeom<TA>::kSmemBytes)) return rc;
+    CUtensorMap tmap_a, tmap_w;
+    if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, TA, pt.a)) return rc;
+    if (const int rc = make_tc3_weight_map(&tmap_w, dW, K, N, pt.w)) return rc;
+    const long tiles = static_cast<long>((M + TA - 1) / TA) * ((N + tb200::kTc3TileW - 1) / tb200::kTc3TileW);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * 2 * cut));
+    cfg.blockDim = dim3(tb200::kSpThreads);
+    cfg.dynamicSmemBytes = tb200::SpGeom<TA>::kSmemBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(2 * cut);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap_a, tmap_w, M, K, N, cut, d_status, epi));
+    return TERNIX_B200_OK;
+}
+struct SplitPlan {
+    int rows, cut;             // rows 0: the persistent form serves the product better
+};
+SplitPlan plan_split(int M, int K, int N) {
+    const Options& o = options();
+    const int blocks = (K + tb200::kTc3BK - 1) / tb200::kTc3BK;
+    if (o.split_rows == 64 || o.split_rows == 128 || o.split_rows == 256)
+        return {o.split_rows, o.split_cut >= 4 && blocks >= 4 ? 4 : o.split_cut >= 2 && blocks >= 2 ? 2 : 1};
+    return {0, 0};
+}
+
 // The kernels that read through TMA, on operands that it can describe (pitches in `pt`).  kernel: TERNIX_B200_KERNEL_*,
 // not AUTO or GENERIC.
+template <typename Epi>
 int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Pitches& pt,
-                     const tb200::FusedEpilogue& epi, int32_t* d_status, cudaStream_t st) {
+                     const Epi& epi, int32_t* d_status, cudaStream_t st) {
     switch (kernel) {
         case TERNIX_B200_KERNEL_GEMV:
             g_last_launched = TERNIX_B200_LAUNCHED_GEMV;
@@ -1212,6 +1255,13 @@ int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int
             return launch_skinny_t<128, false>(prob, sg, nullptr, nullptr, nullptr, grid, nullptr, 0, d_status, st, epi);
         }
         default: {
+            const SplitPlan sp = plan_split(M, K, N);
+            if (sp.rows) {
+                g_last_launched = TERNIX_B200_LAUNCHED_GEMM_SPLIT;
+                if (sp.rows == 64) return launch_gemm_split_t<64>(dA, dW, M, K, N, pt, sp.cut, epi, d_status, st);
+                if (sp.rows == 128) return launch_gemm_split_t<128>(dA, dW, M, K, N, pt, sp.cut, epi, d_status, st);
+                return launch_gemm_split_t<256>(dA, dW, M, K, N, pt, sp.cut, epi, d_status, st);
+            }
             g_last_launched = TERNIX_B200_LAUNCHED_GEMM_TC3;
             CUtensorMap tmap_a, tmap_w;
             if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, tc3_tile_rows(M), pt.a)) return rc;
@@ -1223,7 +1273,8 @@ int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int
 
 // Operands that the TMA unit cannot describe (ragged pitch or unaligned base), product too large for the generic kernel:
 // copy them to pitches of 16 bytes in stream-ordered scratch and run the kernel that the aligned problem would get.
-int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const tb200::FusedEpilogue& epi,
+template <typename Epi>
+int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Epi& epi,
                               int32_t* d_status, cudaStream_t st) {
     const long long a_pitch = (K + 15LL) / 16 * 16, w_pitch = (N / 4 + 15LL) / 16 * 16;
     cudaMemPool_t pool = nullptr;
@@ -1262,7 +1313,8 @@ int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K,
     return rc;
 }
 
-int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, int N, const tb200::FusedEpilogue& epi,
+template <typename Epi>
+int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Epi& epi,
                  int32_t* d_status, cudaStream_t st) {
     switch (kernel) {
         case TERNIX_B200_KERNEL_GEMV: if (!gemv_ok(dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
@@ -1482,6 +1534,7 @@ const char* ternix_b200_launched_kernel_name(int id) {
         case TERNIX_B200_LAUNCHED_SKINNY_TC: return "ternary_skinny_tc_kernel";
         case TERNIX_B200_LAUNCHED_GEMM_TC2: return "ternary_gemm_tc2_kernel";
         case TERNIX_B200_LAUNCHED_GEMM_TC3: return "ternary_gemm_tc3_kernel";
+        case TERNIX_B200_LAUNCHED_GEMM_SPLIT: return "ternary_gemm_split_kernel";
         default: return "none";
     }
 }
@@ -2592,21 +2645,23 @@ int ternix_b200_matmul_fused(const int8_t* dA, const uint8_t* dW, const ternix_b
     if (!aligned(dY, static_cast<uintptr_t>(e)) || !aligned(ep->residual, static_cast<uintptr_t>(e)) || !aligned(ep->row_scale, 4) ||
         !aligned(ep->col_scale, 4))
         return TERNIX_B200_ERR_INVALID_ARG;
-    tb200::FusedEpilogue epi{};
-    epi.row_scale = ep->row_scale;
-    epi.col_scale = ep->col_scale;
-    epi.w_scale = ep->w_scale;
-    epi.bias = ep->bias;
-    epi.bias_dtype = ep->bias_dtype;
-    epi.act = ep->activation;
-    epi.residual = ep->residual;
-    epi.ldr = ep->ldr;
-    epi.out = dY;
-    epi.ldo = ldy;
-    epi.out_dtype = ep->out_dtype;
-    auto vec = [&](const void* p, long long ld) { return aligned(p, static_cast<uintptr_t>(4 * e)) && (M == 1 || ld % 4 == 0); };
-    epi.vec4 = vec(dY, ldy) && (!ep->residual || vec(ep->residual, ep->ldr));
-    return launch_fused(kernel, dA, dW, M, K, N, epi, d_status, static_cast<cudaStream_t>(stream));
+    auto run = [&](auto epi) {
+        epi.row_scale = ep->row_scale;
+        epi.col_scale = ep->col_scale;
+        epi.w_scale = ep->w_scale;
+        epi.bias = ep->bias;
+        epi.bias_dtype = ep->bias_dtype;
+        epi.act = ep->activation;
+        epi.residual = ep->residual;
+        epi.ldr = ep->ldr;
+        epi.out = dY;
+        epi.ldo = ldy;
+        epi.out_dtype = ep->out_dtype;
+        auto vec = [&](const void* p, long long ld) { return aligned(p, static_cast<uintptr_t>(4 * e)) && (M == 1 || ld % 4 == 0); };
+        epi.vec4 = vec(dY, ldy) && (!ep->residual || vec(ep->residual, ep->ldr));
+        return launch_fused(kernel, dA, dW, M, K, N, epi, d_status, static_cast<cudaStream_t>(stream));
+    };
+    return ep->out_dtype == TERNIX_B200_DTYPE_F32 ? run(tb200::FusedEpilogue<true>{}) : run(tb200::FusedEpilogue<false>{});
 }
 
 int ternix_b200_matmul_dequant(const int8_t* dA, const uint8_t* dW, void* const* dY_list, int n_dest,
