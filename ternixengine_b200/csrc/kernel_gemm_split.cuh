@@ -19,8 +19,9 @@
 
 namespace tb200 {
 
-constexpr int kSpWarps = 20, kSpThreads = kSpWarps * 32;          // 0-3 control, 4-11 expanders, 12-19 accumulator readers
-constexpr int kSpFirstExpandWarp = 4, kSpFirstReadWarp = 12;
+constexpr int kSpTurns = 4;                                       // expander warps per lane quarter: they take the stages in turn
+constexpr int kSpFirstExpandWarp = 4;                             // warps 0-3 control; the expanders also read the accumulator
+constexpr int kSpWarps = kSpFirstExpandWarp + 4 * kSpTurns, kSpThreads = kSpWarps * 32;
 constexpr int kSpMaxCut = 4;                                      // pairs of a cluster: 8 CTAs, the portable limit
 constexpr int kSpWStages = 8, kSpTStages = 4;                     // packed-weight ring; operand ring in tensor memory
 template <int TA>
@@ -29,11 +30,14 @@ struct SpGeom {
     static constexpr int kRowsPerCta = TA / 2;
     static constexpr int kActBox = kRowsPerCta * 128;             // rows x 128 K-bytes, 128-byte swizzle
     static constexpr int kActBytes = 2 * kActBox;
-    static constexpr int kStages = TA == 256 ? 4 : TA == 128 ? 6 : 8;
+    static constexpr int kStages = TA == 256 ? 4 : 8;
+    // Two MMA issuers take the k-blocks in turn, each into an accumulator of its own, where two of them fit beside the operand
+    // ring (256 columns): a k-block costs one thread 8 MMAs of 60-90 cycles whatever their N, a commit of 180 and a wait.
+    static constexpr int kIssuers = TA <= 128 ? 2 : 1;
     static constexpr int kPartBytes = TA * 128 * 4;               // this CTA's half of the tile as int32
     static_assert(kStages * kActBytes >= kPartBytes, "the partial tile lies over the activation ring");
-    // an expander warp meets every phase of the barriers it waits on (two warps per lane quarter take the stages in turn)
-    static_assert(kStages % 2 == 0 && kStages >= kSpTStages && kSpTStages % 2 == 0 && kSpWStages % 2 == 0, "ring sizes");
+    // an expander warp meets every phase of the barriers it waits on
+    static_assert(kStages % kSpTurns == 0 && kStages >= kSpTStages && kSpTStages % kSpTurns == 0 && kSpWStages % kSpTurns == 0, "ring sizes");
     static constexpr size_t kSmemBytes = 1024 + size_t(kStages) * kActBytes + size_t(kSpWStages) * kTc3WpBytes + 512;
     static constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(TA >> 3) << 17) | (uint32_t(256 >> 4) << 24);
 };
@@ -76,44 +80,60 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
         for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int s = 0; s < TS; ++s) mbar_init(&ready[s], 2 * 4);
         for (int s = 0; s < WS; ++s) { mbar_init(&w_full[s], 1); mbar_init(&w_empty[s], 4); }
-        mbar_init(acc_full, 1);
-        mbar_init(drain, 1);
+        mbar_init(acc_full, G::kIssuers);
+        mbar_init(drain, G::kIssuers);
         *abort_flag = 0;
         mbar_init_fence();
     }
+    auto load_act = [&](uint32_t it) {
+        const uint32_t s = it % S;
+        mbar_arrive_expect_tx(&full[s], G::kActBytes);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            tma_load_2d(sAct + s * G::kActBytes + j * G::kActBox, &tmap_a, (kb0 + static_cast<int>(it)) * kTc3BK + j * 128,
+                        row0 + static_cast<int>(half) * G::kRowsPerCta, &full[s]);
+    };
+    auto load_weights = [&](uint32_t it) {
+        const uint32_t sw = it % WS;
+        mbar_arrive_expect_tx(&w_full[sw], kTc3WpBytes);
+        tma_load_2d(sWp + sw * kTc3WpBytes, &tmap_w, col0 / 4, (kb0 + static_cast<int>(it)) * kTc3BK, &w_full[sw]);
+    };
     if (warp == 1) {
         tmem_alloc_pair<512>(tmem_slot);
         tmem_relinquish_pair();
     }
+    __syncwarp();
     tc_fence_before_sync();
-    cluster_sync_all();
+    __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    // The CTAs of the cluster meet here, but nobody waits for the others yet: loads and expansion touch this CTA only.  The
+    // first thing that needs a peer is the arrival on the leader's `ready` barrier.
+    cluster_arrive();
 
     if (warp == 0) {
         // ================================================================ activations
         if (lane == 0) {
-            tma_prefetch_desc(&tmap_a);
             uint32_t it = 0;
             for (; it < n_kb; ++it) {
-                const uint32_t s = it % S;
-                if (!mbar_wait_backoff(&empty[s], ((it / S) & 1) ^ 1, abort_flag, 32)) break;
-                mbar_arrive_expect_tx(&full[s], G::kActBytes);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    tma_load_2d(sAct + s * G::kActBytes + j * G::kActBox, &tmap_a, (kb0 + static_cast<int>(it)) * kTc3BK + j * 128,
-                                row0 + static_cast<int>(half) * G::kRowsPerCta, &full[s]);
+                if (!mbar_wait_backoff(&empty[it % S], ((it / S) & 1) ^ 1, abort_flag, 32)) break;
+                load_act(it);
             }
-            if (it < n_kb) {
+            if (*abort_flag) {
                 const uint32_t first = it > static_cast<uint32_t>(S) ? it - S : 0;
                 for (uint32_t j = first; j < it; ++j) mbar_drain(&full[j % S], (j / S) & 1);
             }
         }
-    } else if (warp == 1) {
-        // ================================================================ MMA issuer (leader CTA of the pair)
-        if (leader && lane == 0) {
+        __syncwarp();
+        cluster_wait();
+    } else if (warp == 1 || warp == 3) {
+        // ================================================================ MMA issuers (leader CTA of the pair)
+        const uint32_t who = warp >> 1;                       // warps 1 and 3
+        cluster_wait();
+        if (leader && lane == 0 && who < static_cast<uint32_t>(G::kIssuers)) {
             bool ok = true;
-            for (uint32_t it = 0; it < n_kb; ++it) {
+            const uint32_t acc = tmem_base + who * TA;
+            for (uint32_t it = who; it < n_kb; it += G::kIssuers) {
                 const uint32_t s = it % S, ts = it % TS;
                 if (!mbar_wait(&ready[ts], (it / TS) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after_sync();
@@ -122,7 +142,7 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
 #pragma unroll
                 for (int g = 0; g < kTc3BK / 32; ++g) {
                     const uint64_t db = umma_desc_sw128(act_addr + (g >> 2) * G::kActBox + (g & 3) * 32, 16, 1024);
-                    tc_mma_i8_pair_tmem_a(tmem_base, a_col + 8 * g, db, G::kIdesc, (it != 0 || g != 0) ? 1u : 0u);
+                    tc_mma_i8_pair_tmem_a(acc, a_col + 8 * g, db, G::kIdesc, (it != who || g != 0) ? 1u : 0u);
                 }
                 tc_commit_pair_both(&empty[s], pair_mask);
             }
@@ -133,20 +153,19 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
     } else if (warp == 2) {
         // ================================================================ packed weights
         if (lane == 0) {
-            tma_prefetch_desc(&tmap_w);
             uint32_t it = 0;
             for (; it < n_kb; ++it) {
-                const uint32_t sw = it % WS;
-                if (!mbar_wait_backoff(&w_empty[sw], ((it / WS) & 1) ^ 1, abort_flag, 32)) break;
-                mbar_arrive_expect_tx(&w_full[sw], kTc3WpBytes);
-                tma_load_2d(sWp + sw * kTc3WpBytes, &tmap_w, col0 / 4, (kb0 + static_cast<int>(it)) * kTc3BK, &w_full[sw]);
+                if (!mbar_wait_backoff(&w_empty[it % WS], ((it / WS) & 1) ^ 1, abort_flag, 32)) break;
+                load_weights(it);
             }
-            if (it < n_kb) {
+            if (*abort_flag) {
                 const uint32_t first = it > static_cast<uint32_t>(WS) ? it - WS : 0;
                 for (uint32_t j = first; j < it; ++j) mbar_drain(&w_full[j % WS], (j / WS) & 1);
             }
         }
-    } else if (warp >= kSpFirstExpandWarp && warp < kSpFirstReadWarp) {
+        __syncwarp();
+        cluster_wait();
+    } else if (warp >= kSpFirstExpandWarp) {
         // ================================================================ expanders, as in kernel_gemm_tc3.cuh
         const uint32_t q = warp & 3;
         const uint32_t slot = (warp - kSpFirstExpandWarp) >> 2;
@@ -155,7 +174,8 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
         const bool odd = (q & 1) != 0;
         const uint32_t wp_sa = smem_u32(sWp);
         const uint32_t t_lane = (q * 32) << 16;
-        for (uint32_t it = slot; it < n_kb; it += 2) {
+        bool met = false;
+        for (uint32_t it = slot; it < n_kb; it += kSpTurns) {
             const uint32_t s = it % S, ts = it % TS, sw = it % WS;
             if (!mbar_wait_backoff(&w_full[sw], (it / WS) & 1, abort_flag, 32)) break;
             const uint32_t wp = wp_sa + sw * kTc3WpBytes + ld_off;
@@ -186,29 +206,38 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
             tmem_st_wait();
             tc_fence_before_sync();
             if (q == 0 && !mbar_wait_backoff(&full[s], (it / S) & 1, abort_flag, 32)) break;
+            if (!met) cluster_wait();
+            met = true;
             __syncwarp();
             if (lane == 0) {
                 if (leader) mbar_arrive(&ready[ts]);
                 else mbar_arrive_remote(&ready[ts], lead);
             }
         }
-    } else if (warp >= kSpFirstReadWarp) {
+        if (!met) cluster_wait();
         // ================================================================ partial sums: tensor memory -> shared memory
         // The tile's residual comes into L2 meanwhile: the rows this CTA will finish, one per thread.
         const int share = TA / cut, first = row0 + static_cast<int>(pair) * share;
-        const int mine = static_cast<int>(threadIdx.x) - kSpFirstReadWarp * 32;
+        const int mine = static_cast<int>(threadIdx.x) - kSpFirstExpandWarp * 32;
         if (epi.residual && mine < share && first + mine < M && col0 < N) epi.prefetch_residual(first + mine, col0, min(128, N - col0));
         __syncwarp();
-        const uint32_t q = warp & 3, colp = q * 32 + 4 * (lane & 7) + (lane >> 3);       // the expanders' column numbering
+        const uint32_t colp = q * 32 + 4 * (lane & 7) + (lane >> 3);       // the column numbering above
         const uint32_t part = smem_u32(sAct);
         if (mbar_wait_backoff(acc_full, 0, abort_flag, 64)) {
             tc_fence_after_sync();
             __syncwarp();
 #pragma unroll 1
-            for (int c = (warp - kSpFirstReadWarp) >> 2; c < TA / 32; c += 2) {
+            for (int c = static_cast<int>(slot); c < TA / 32; c += kSpTurns) {
                 uint32_t r[32];
                 tmem_ld_32x32(tmem_base + ((q * 32) << 16) + 32 * c, r);
                 tmem_ld_wait();
+                if (G::kIssuers > 1 && n_kb > 1) {            // an issuer without a k-block left its accumulator untouched
+                    uint32_t r1[32];
+                    tmem_ld_32x32(tmem_base + ((q * 32) << 16) + TA + 32 * c, r1);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[j] += r1[j];
+                }
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     sts_u32(part + (((32 * c + j) * 128 + colp) << 2), static_cast<uint32_t>(static_cast<int32_t>(r[j]) >> 6));

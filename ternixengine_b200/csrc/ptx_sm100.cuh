@@ -221,6 +221,9 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void cluster_sync_threads() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// The barrier in two halves, for work that needs no peer in between; every thread executes both.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // Address of `smem_addr` (a shared::cta address of this CTA's layout) inside CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t dsmem_map(uint32_t smem_addr, uint32_t rank) {
     uint32_t r;
