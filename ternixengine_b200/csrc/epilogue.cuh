@@ -54,19 +54,6 @@ __device__ __forceinline__ float rcp_approx(float x) {
 __device__ __forceinline__ float logistic_times(float v, float u) {
     return v * rcp_approx(1.0f + exp2_approx(-1.44269504f * u));
 }
-// v (1 + erf(v / sqrt 2)) / 2 through erfc: Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26,
-//   erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) + e,  t = 1 / (1 + p x),  x >= 0,  |e| <= 1.5e-7,
-// which is what fp32 resolves next to 1; a third of the instructions of the library's erf.
-__device__ __forceinline__ float gelu(float v) {
-    const float x = fabsf(v) * 0.70710678f;
-    const float t = rcp_approx(fmaf(0.3275911f, x, 1.0f));
-    float s = fmaf(1.061405429f, t, -1.453152027f);
-    s = fmaf(s, t, 1.421413741f);
-    s = fmaf(s, t, -0.284496736f);
-    s = fmaf(s, t, 0.254829592f);
-    const float half_erfc = 0.5f * (s * t) * exp2_approx(-1.44269504f * (x * x));
-    return v * (v < 0.0f ? half_erfc : 1.0f - half_erfc);
-}
 // act(v) on N values at once: the choice is the same for the whole launch, so it is made once per N values.  A NaN stays
 // a NaN in every activation.
 template <int N>
@@ -89,7 +76,7 @@ __device__ __forceinline__ void activate(int act, float (&v)[N]) {
             break;
         case kActGelu:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = gelu(v[i]);
+            for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
             break;
         case kActGeluTanh:       // 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
 #pragma unroll

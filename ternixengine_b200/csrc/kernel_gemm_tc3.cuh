@@ -155,6 +155,8 @@ constexpr size_t tc3_smem_bytes() {
 }
 static_assert(tc3_smem_bytes<128>() <= 227 * 1024 && tc3_smem_bytes<256>() <= 227 * 1024, "shared memory: 227 KB per CTA");
 constexpr size_t kTc3SmemBytes = tc3_smem_bytes<256>();
+constexpr size_t kTc3FusedSmem = 1024;            // the fused epilogue's row scales, behind the barriers
+static_assert(kTc3SmemBytes + kTc3FusedSmem <= 227 * 1024, "shared memory: 227 KB per CTA");
 
 __device__ __forceinline__ void tc_mma_i8_pair_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
                                                       uint32_t accumulate) {
@@ -270,9 +272,11 @@ __device__ __forceinline__ void sts_u16(uint32_t saddr, uint16_t v) {
 // pair's MMAs are half as long, and tensor-memory columns 0-255 hold TWO accumulators: the MMAs of the next tile run
 // while the epilogue warps empty the previous one.  The shared-memory ring is then deeper than the operand ring in
 // tensor memory (a stage passes in half the time, the latency of a TMA load stays what it is).
-// Epi = FusedEpilogue: the finished sums go through the staging buffer as int32, and the four warps of an epilogue group
-// read it back row by row, four columns to a lane: scales, bias, activation and residual in registers, coalesced loads of
-// the residual and stores of the output (256 bytes of bfloat16 per row and warp) at any pitch, without a TMA view.
+// Epi = FusedEpilogue: an epilogue warp takes its accumulator registers through scales, bias and activation in place and
+// writes them to the staging buffer as fp32; the group's four warps read that back row by row, four columns to a lane,
+// for coalesced loads of the residual and stores of the output (256 bytes of bfloat16 per row and warp) at any pitch,
+// without a TMA view.  Eight warps per CTA hold the accumulator, so what they do is bound by latency, not by issue slots:
+// done row by row on four values at a time (the first form) an epilogue of 256 x 256 took 12 us and K = 2560 waited for it.
 template <bool kGrouped, bool kBf16 = false, int TA = kTc3TileA, typename Epi = StoreInt32>
 __global__ void __launch_bounds__(kTc3Threads, 1)
 ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
@@ -527,6 +531,7 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         const int eg = (warp - kTc3FirstEpilogueWarp) >> 2;             // group: takes steps eg, eg + groups, ...
         const bool elected = ((warp - kTc3FirstEpilogueWarp) & 3) == 0 && lane == 0;
         const uint32_t epi_sa = smem_u32(sEpi);
+        const uint32_t rs_sa = smem_u32(bars) + 512 + eg * 512;         // (fused) the group's row scales, 128 of them
         uint32_t lt = 0, step = 0;                                      // step: steps taken by this group so far
         bool ok = true;
         Tc3Walk<kGrouped> w = make_walk();
@@ -543,8 +548,17 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             const long long ldc = w.ldc;
             int32_t* C = w.C;
             const uint32_t ab = lt % BUFS;
+            float col_s = 0.0f, col_b = 0.0f;
             if constexpr (Epi::kFused) {
-                // the tile's residual into L2 while its MMAs run: one row of it per thread
+                // While the tile's MMAs run: this lane's column scale and bias, the group's row scales into shared memory (step
+                // i of group eg has rows 32 (eg + 2i) ..; every reader is past them: the steps below end in the other pass),
+                // and the tile's residual into L2, one row of it per thread.
+                const int t = static_cast<int>((warp & 3) * 32 + lane), c = w.w_t * kTc3TileW + rank * 128 + static_cast<int>(colp);
+                if (t < 32 * kSteps) {
+                    const int row = a_t * TA + 32 * (eg + kTc3EpiGroups * (t >> 5)) + (t & 31);
+                    sts_u32(rs_sa + 4 * t, row < M ? __float_as_uint(__ldg(epi.row_scale + row)) : 0u);
+                }
+                if (c < N) { col_s = epi.column_scale(c); col_b = epi.column_bias(c); }
                 const int row = a_t * TA + static_cast<int>((warp - kTc3FirstEpilogueWarp) * 32 + lane);
                 const int col = w.w_t * kTc3TileW + rank * 128;
                 if (epi.residual && row < M && row < (a_t + 1) * TA && col < N) epi.prefetch_residual(row, col, min(128, N - col));
@@ -573,12 +587,22 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
                 const int row0 = a_t * TA + 32 * c;
                 if constexpr (Epi::kFused) {
+                    // Scales, bias and activation in place, in the accumulator's own layout (lane = column, registers = rows):
+                    // 32 independent chains and no registers beside the accumulator's.
+                    float (&v)[32] = reinterpret_cast<float (&)[32]>(r[i]);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        sts_u32(buf + ((j * 128 + colp) << 2), static_cast<uint32_t>(static_cast<int32_t>(r[i][j]) >> 6));
-                    // Everything the step needs from global memory is requested here, before the barrier, so that its
-                    // latency is met once per step: the residual of this warp's eight rows (four at a time in float32),
-                    // their scales (lane j holds row j's) and, for the tile, the columns' scales and biases.
+                    for (int j = 0; j < 32; j += 4) {
+                        const uint4 rs = lds_v4(rs_sa + (32 * i + j) * 4);
+                        v[j] = epi.linear(static_cast<int32_t>(r[i][j]) >> 6, __uint_as_float(rs.x), col_s, col_b);
+                        v[j + 1] = epi.linear(static_cast<int32_t>(r[i][j + 1]) >> 6, __uint_as_float(rs.y), col_s, col_b);
+                        v[j + 2] = epi.linear(static_cast<int32_t>(r[i][j + 2]) >> 6, __uint_as_float(rs.z), col_s, col_b);
+                        v[j + 3] = epi.linear(static_cast<int32_t>(r[i][j + 3]) >> 6, __uint_as_float(rs.w), col_s, col_b);
+                    }
+                    activate(epi.act, v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sts_u32(buf + ((j * 128 + colp) << 2), __float_as_uint(v[j]));
+                    // Row by row from here: a warp has eight rows, a lane four columns.  The residual is requested before the
+                    // barrier, so that its latency is met once per step (four rows at a time in float32).
                     const int col = col0 + 4 * lane, first = row0 + 8 * static_cast<int>(q);
                     constexpr int kAhead = sizeof(typename Epi::Raw) == 8 ? 8 : 4;
                     typename Epi::Raw raw[kAhead];
@@ -587,36 +611,14 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                         raw[j] = typename Epi::Raw{};
                         if (col < N && first + j < M) raw[j] = epi.load_residual4(first + j, col);
                     }
-                    const float rs_lane = first + (lane & 7) < M ? __ldg(epi.row_scale + first + (lane & 7)) : 0.0f;
-                    float cs[4], b[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        cs[x] = col < N ? epi.column_scale(col + x) : 0.0f;
-                        b[x] = col < N ? epi.column_bias(col + x) : 0.0f;
-                    }
                     asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float v[16];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint4 sum = lds_v4(buf + ((8 * q + 4 * h + j) * 128 + 4 * lane) * 4);
-                            const float rs = __shfl_sync(0xffffffffu, rs_lane, 4 * h + j);
-                            v[4 * j] = epi.linear(static_cast<int32_t>(sum.x), rs, cs[0], b[0]);
-                            v[4 * j + 1] = epi.linear(static_cast<int32_t>(sum.y), rs, cs[1], b[1]);
-                            v[4 * j + 2] = epi.linear(static_cast<int32_t>(sum.z), rs, cs[2], b[2]);
-                            v[4 * j + 3] = epi.linear(static_cast<int32_t>(sum.w), rs, cs[3], b[3]);
-                        }
-                        activate(epi.act, v);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (col < N && first + 4 * h + j < M) epi.finish4(first + 4 * h + j, col, v + 4 * j, raw[(4 * h + j) % kAhead]);
-                        if constexpr (kAhead == 4) {
-                            if (h == 0) {
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    if (col < N && first + 4 + j < M) raw[j] = epi.load_residual4(first + 4 + j, col);
-                            }
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 y = lds_v4(buf + ((8 * q + j) * 128 + 4 * lane) * 4);
+                        const float f[4] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w)};
+                        if (col < N && first + j < M) {
+                            epi.finish4(first + j, col, f, raw[j % kAhead]);
+                            if (kAhead == 4 && j < 4 && first + j + 4 < M) raw[j % kAhead] = epi.load_residual4(first + j + 4, col);
                         }
                     }
                     __syncwarp();

@@ -617,14 +617,15 @@ int make_tc3_store_map(CUtensorMap* out, int32_t* dC, int M, int N, long long ld
 template <int TA, typename Epi>
 int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const tb200::Tc3Stores& stores, int32_t* dC0,
                            int M, int K, int N, long long ldc, int32_t* d_status, const Epi& epi, cudaStream_t st) {
-    if (const int arc = ensure_smem_attr<tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>>(tb200::tc3_smem_bytes<TA>())) return arc;
+    constexpr size_t smem = tb200::tc3_smem_bytes<TA>() + (Epi::kFused ? tb200::kTc3FusedSmem : 0);
+    if (const int arc = ensure_smem_attr<tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>>(smem)) return arc;
     const long tiles = static_cast<long>((M + TA - 1) / TA) * ((N + tb200::kTc3TileW - 1) / tb200::kTc3TileW);
     const long max_pairs = sm_count() / 2;
     const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * pairs, 1, 1);
     cfg.blockDim = dim3(tb200::kTc3Threads, 1, 1);
-    cfg.dynamicSmemBytes = tb200::tc3_smem_bytes<TA>();
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
