@@ -613,12 +613,19 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     }
                     asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint4 y = lds_v4(buf + ((8 * q + j) * 128 + 4 * lane) * 4);
-                        const float f[4] = {__uint_as_float(y.x), __uint_as_float(y.y), __uint_as_float(y.z), __uint_as_float(y.w)};
-                        if (col < N && first + j < M) {
-                            epi.finish4(first + j, col, f, raw[j % kAhead]);
-                            if (kAhead == 4 && j < 4 && first + j + 4 < M) raw[j % kAhead] = epi.load_residual4(first + j + 4, col);
+                    for (int h = 0; h < 8; h += 4) {
+                        uint4 y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) y[j] = lds_v4(buf + ((8 * q + h + j) * 128 + 4 * lane) * 4);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float f[4] = {__uint_as_float(y[j].x), __uint_as_float(y[j].y), __uint_as_float(y[j].z), __uint_as_float(y[j].w)};
+                            if (col < N && first + h + j < M) epi.finish4(first + h + j, col, f, raw[(h + j) % kAhead]);
+                        }
+                        if (kAhead == 4 && h == 0) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (col < N && first + 4 + j < M) raw[j] = epi.load_residual4(first + 4 + j, col);
                         }
                     }
                     __syncwarp();
