@@ -297,7 +297,8 @@ int ternix_b200_glu_quantize(const void *dGate, long long ldg, const void *dUp, 
  * NULL (column scales let projections with scales of their own share one weight matrix).  bias and residual may be NULL;
  * bias is [N] of bias_dtype; residual has the output's type and row pitch ldr >= N and may be dY itself (not a shifted
  * view of it).  dY has row pitch ldy >= N.  Sums beyond 2^24 (|c| can reach 128 K) round once on their way to fp32.
- * Shapes, alignment, `kernel` and d_status as in ternix_b200_matmul_ex; GEMM_TC is the tensor-memory kernel.  K == 0 gives
+ * Shapes, alignment, `kernel` and d_status as in ternix_b200_matmul_ex; GEMM_TC is the tensor-memory kernel in its persistent
+ * or its cut form, SKINNY_TC has no fused form (TERNIX_B200_ERR_UNSUPPORTED).  K == 0 gives
  * y = act(bias) + residual.  A product with a ragged K, N or unaligned operand that is too large for the generic kernel
  * takes an aligned copy of its operands from the library's pool (ternix_b200_release_cached_memory), on `stream`. */
 typedef struct ternix_b200_epilogue {

@@ -220,13 +220,12 @@ struct SkWalk {
     }
 };
 
-template <int NB, bool kGrouped, typename Epi = StoreInt32>
+template <int NB, bool kGrouped>
 __global__ void __launch_bounds__(SkGeom<NB>::kThreads, 1)
 ternary_skinny_tc_kernel(const __grid_constant__ SkProblem single, const SkSingle sg,
                          const SkProblem* __restrict__ probs, const SkItem* __restrict__ items,
                          const int* __restrict__ cta_first, int* __restrict__ flags, int epoch,
-                         int32_t* __restrict__ status, const Epi epi) {
-    static_assert(!(kGrouped && Epi::kFused), "the fused epilogue is built for single products");
+                         int32_t* __restrict__ status) {
     using G = SkGeom<NB>;
     constexpr int TS = G::kTStages, AS = G::kAStages, WS = G::kWStages, BUFS = G::kAccBufs;
     extern __shared__ uint8_t smem_raw[];
@@ -534,28 +533,6 @@ ternary_skinny_tc_kernel(const __grid_constant__ SkProblem single, const SkSingl
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&acc_empty[ab * 2 + h]);
-                    }
-                    if constexpr (Epi::kFused) {
-                        // whole-K items only (the host plans no shared blocks): every sum is final here
-                        const float cs = col < N ? epi.column_scale(col) : 0.0f, b = col < N ? epi.column_bias(col) : 0.0f;
-#pragma unroll
-                        for (int c = 0; c < kBatch; ++c) {
-                            const int first = 16 * (c0 + c);
-                            const float rs_lane = first + (lane & 15) < M ? __ldg(epi.row_scale + first + (lane & 15)) : 0.0f;
-#pragma unroll
-                            for (int g = 0; g < 16; g += 8) {
-                                float v[8];
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    v[j] = epi.linear(static_cast<int32_t>(r[c][g + j]) >> 6, __shfl_sync(0xffffffffu, rs_lane, g + j), cs, b);
-                                activate(epi.act, v);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    if (first + g + j < M && col < N) epi.finish(first + g + j, col, v[j]);
-                            }
-                        }
-                        __syncwarp();          // the tensor-memory instructions of the next batch want the warp together
-                        continue;
                     }
                     if (col >= N) continue;
 #pragma unroll

@@ -643,12 +643,11 @@ int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w,
 }
 
 // tmap_a must have been made for tc3_tile_rows(M).
-template <typename Epi = tb200::StoreInt32>
 int launch_gemm_tc3_maps(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const tb200::Tc3Stores& stores, int32_t* dC0,
-                         int M, int K, int N, long long ldc, int32_t* d_status, cudaStream_t st, const Epi& epi = {}) {
+                         int M, int K, int N, long long ldc, int32_t* d_status, cudaStream_t st) {
     if (tc3_tile_rows(M) == 128)
-        return launch_gemm_tc3_maps_t<128>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, epi, st);
-    return launch_gemm_tc3_maps_t<256>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, epi, st);
+        return launch_gemm_tc3_maps_t<128>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, tb200::StoreInt32{}, st);
+    return launch_gemm_tc3_maps_t<256>(tmap_a, tmap_w, stores, dC0, M, K, N, ldc, d_status, tb200::StoreInt32{}, st);
 }
 
 int launch_gemm_tc3(const int8_t* dA, const uint8_t* dW, int32_t* const* dC_list, int n_dest, int M, int K, int N,
@@ -755,13 +754,13 @@ int next_skinny_epoch() {
 int skinny_rows_class(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
 
 int make_skinny_problem(tb200::SkProblem* out, const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N,
-                        long long ldc, int rows_class = 0, const Pitches& pt = {}) {
+                        long long ldc) {
     *out = tb200::SkProblem{};
     int rc = make_tmap_2d(&out->tmap_w, dW, static_cast<uint64_t>(N / 4), static_cast<uint64_t>(K),
-                          static_cast<uint64_t>(pt.w ? pt.w : N / 4), tb200::kSkWpRowBytes, tb200::kSkBK, CU_TENSOR_MAP_SWIZZLE_64B);
+                          static_cast<uint64_t>(N / 4), tb200::kSkWpRowBytes, tb200::kSkBK, CU_TENSOR_MAP_SWIZZLE_64B);
     if (rc) return rc;
-    rc = make_tmap_2d(&out->tmap_a, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(pt.a ? pt.a : K), 128,
-                      rows_class ? rows_class : skinny_rows_class(M), CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tmap_2d(&out->tmap_a, dA, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(K), 128,
+                      skinny_rows_class(M), CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     out->C = dC;
     out->ldc = ldc;
@@ -771,14 +770,14 @@ int make_skinny_problem(tb200::SkProblem* out, const int8_t* dA, const uint8_t* 
     return TERNIX_B200_OK;
 }
 
-template <int NB, bool kGrouped, typename Epi = tb200::StoreInt32>
+template <int NB, bool kGrouped>
 int launch_skinny_t(const tb200::SkProblem& single, const tb200::SkSingle& sg, const tb200::SkProblem* d_probs,
                     const tb200::SkItem* d_items, const int* d_first, int grid, int* d_flags, int epoch,
-                    int32_t* d_status, cudaStream_t st, const Epi& epi = {}) {
-    if (const int arc = ensure_smem_attr<tb200::ternary_skinny_tc_kernel<NB, kGrouped, Epi>>(tb200::SkGeom<NB>::kSmemBytes))
+                    int32_t* d_status, cudaStream_t st) {
+    if (const int arc = ensure_smem_attr<tb200::ternary_skinny_tc_kernel<NB, kGrouped>>(tb200::SkGeom<NB>::kSmemBytes))
         return arc;
-    tb200::ternary_skinny_tc_kernel<NB, kGrouped, Epi><<<grid, tb200::SkGeom<NB>::kThreads, tb200::SkGeom<NB>::kSmemBytes, st>>>(
-        single, sg, d_probs, d_items, d_first, d_flags, epoch, d_status, epi);
+    tb200::ternary_skinny_tc_kernel<NB, kGrouped><<<grid, tb200::SkGeom<NB>::kThreads, tb200::SkGeom<NB>::kSmemBytes, st>>>(
+        single, sg, d_probs, d_items, d_first, d_flags, epoch, d_status);
     TB_CUDA(cudaGetLastError());
     return TERNIX_B200_OK;
 }
@@ -1220,15 +1219,64 @@ int launch_gemm_split_t(const int8_t* dA, const uint8_t* dW, int M, int K, int N
     TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap_a, tmap_w, M, K, N, cut, d_status, epi));
     return TERNIX_B200_OK;
 }
+// Clusters of the cut form that the device holds at once (asked once per device and form).
+template <int TA, typename Epi>
+int split_clusters(int cut) {
+    static std::atomic<int> cache[kMaxDevices][3] = {};
+    std::atomic<int>& slot = cache[current_device()][cut == 4 ? 2 : cut - 1];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    constexpr auto kern = tb200::ternary_gemm_split_kernel<TA, Epi>;
+    if (ensure_smem_attr<kern>(tb200::SpGeom<TA>::kSmemBytes) != TERNIX_B200_OK) return 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * cut));
+    cfg.blockDim = dim3(tb200::kSpThreads);
+    cfg.dynamicSmemBytes = tb200::SpGeom<TA>::kSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(2 * cut);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return 0;
+    }
+    slot.store(n, std::memory_order_relaxed);
+    return n;
+}
 struct SplitPlan {
     int rows, cut;             // rows 0: the persistent form serves the product better
 };
+// Tile rows and cut with the smallest estimate, in microseconds as measured on B200 for 17 to 1500 rows, K 640 to 8192 and
+// N 640 to 28672: a cluster takes a fixed time (launch, first loads, the way out) and one per k-block of its pairs; clusters
+// beyond what the device holds at once come in waves.  The persistent form pays its way in and out once and afterwards the
+// longer of a tile's MMAs and a tile's epilogue.  E.g. 256 x 6912 x 2560: 13.5 us as 128 rows, cut 2; 28.7 us persistent;
+// 1024 x 2560 x 6912: 34.8 us as 256 rows, uncut; 24 us persistent.
+template <typename Epi>
 SplitPlan plan_split(int M, int K, int N) {
     const Options& o = options();
     const int blocks = (K + tb200::kTc3BK - 1) / tb200::kTc3BK;
     if (o.split_rows == 64 || o.split_rows == 128 || o.split_rows == 256)
         return {o.split_rows, o.split_cut >= 4 && blocks >= 4 ? 4 : o.split_cut >= 2 && blocks >= 2 ? 2 : 1};
-    return {0, 0};
+    const long w_tiles = (N + tb200::kTc3TileW - 1) / tb200::kTc3TileW;
+    const long pairs = std::max(1, sm_count() / 2), tc_waves = ((M + 255L) / 256 * w_tiles + pairs - 1) / pairs;
+    double best = 9.6 + 0.58 * blocks + static_cast<double>(tc_waves - 1) * std::max(0.58 * blocks, 7.3);
+    SplitPlan plan{0, 1};
+    for (const int rows : {64, 128, 256}) {
+        const long tiles = (M + rows - 1L) / rows * w_tiles;
+        for (const int cut : {1, 2, 4}) {
+            if (cut > blocks) continue;
+            const int held = rows == 64 ? split_clusters<64, Epi>(cut) : rows == 128 ? split_clusters<128, Epi>(cut) : split_clusters<256, Epi>(cut);
+            if (held <= 0) continue;
+            const double fixed = rows == 64 ? 6.9 : rows == 128 ? (cut == 1 ? 9.0 : 8.3) : (cut == 1 ? 12.6 : 10.6);
+            const double per_block = rows == 64 ? 0.30 : rows == 128 ? 0.31 : 0.55;
+            const double t = static_cast<double>((tiles + held - 1) / held) * (fixed + per_block * ((blocks + cut - 1) / cut));
+            if (t < best) { best = t; plan = {rows, cut}; }
+        }
+    }
+    return plan;
 }
 
 // The kernels that read through TMA, on operands that it can describe (pitches in `pt`).  kernel: TERNIX_B200_KERNEL_*,
@@ -1243,20 +1291,8 @@ int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int
         case TERNIX_B200_KERNEL_DECODE_MMA:
             g_last_launched = TERNIX_B200_LAUNCHED_DECODE_MMA;
             return launch_decode_mma(dA, dW, nullptr, M, K, N, N, d_status, st, epi, pt);
-        case TERNIX_B200_KERNEL_SKINNY_TC: {
-            // built for 64 and 128 rows (the dispatch never sends it fewer than 33); whole-K items, so no flags
-            g_last_launched = TERNIX_B200_LAUNCHED_SKINNY_TC;
-            const int rows = M <= 64 ? 64 : 128;
-            tb200::SkProblem prob;
-            if (const int rc = make_skinny_problem(&prob, dA, dW, nullptr, M, K, N, N, rows, pt)) return rc;
-            tb200::SkSingle sg{};
-            int grid = 0;
-            plan_skinny(K, N, false, 0, &sg, &grid);
-            if (rows == 64) return launch_skinny_t<64, false>(prob, sg, nullptr, nullptr, nullptr, grid, nullptr, 0, d_status, st, epi);
-            return launch_skinny_t<128, false>(prob, sg, nullptr, nullptr, nullptr, grid, nullptr, 0, d_status, st, epi);
-        }
         default: {
-            const SplitPlan sp = plan_split(M, K, N);
+            const SplitPlan sp = plan_split<Epi>(M, K, N);
             if (sp.rows) {
                 g_last_launched = TERNIX_B200_LAUNCHED_GEMM_SPLIT;
                 if (sp.rows == 64) return launch_gemm_split_t<64>(dA, dW, M, K, N, pt, sp.cut, epi, d_status, st);
@@ -1265,11 +1301,26 @@ int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int
             }
             g_last_launched = TERNIX_B200_LAUNCHED_GEMM_TC3;
             CUtensorMap tmap_a, tmap_w;
-            if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, tc3_tile_rows(M), pt.a)) return rc;
+            if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, 256, pt.a)) return rc;
             if (const int rc = make_tc3_weight_map(&tmap_w, dW, K, N, pt.w)) return rc;
-            return launch_gemm_tc3_maps(tmap_a, tmap_w, tb200::Tc3Stores{}, nullptr, M, K, N, N, d_status, st, epi);
+            return launch_gemm_tc3_maps_t<256>(tmap_a, tmap_w, tb200::Tc3Stores{}, nullptr, M, K, N, N, d_status, epi, st);
         }
     }
+}
+
+// Which kernel takes a fused product.  One row: the GEMV, unless the weights are so many (24 MB) that the clustered
+// mma.sync kernel's streaming pays (8192 x 28672: 23.8 against 18.1 us; 4096 x 11008: 7.7 against 9.0).  Two rows of few
+// weights likewise (2560 x 2560: 4.9 against 6.1 us).  Up to 8 rows mma.sync, which reads the weights once at one row group;
+// from 9 rows (two row groups' worth of instructions) the prefill forms, as soon as one wave of clusters covers N
+// (16 x 6912 x 2560: 9.0 against 12.9 us; 16 x 8192 x 28672, two waves: 31.8 against 27.5), and from 17 rows always.
+int select_fused(const void* dA, const void* dW, int M, int K, int N) {
+    const double w_bytes = static_cast<double>(K) * N / 4;
+    const bool mma = decode_mma_ok(dA, dW, M, K, N);
+    if (gemv_ok(dW, M, K, N) && (M == 1 || (M == 2 && w_bytes <= 6e6) || !mma) && !(mma && w_bytes >= 24e6))
+        return TERNIX_B200_KERNEL_GEMV;
+    if (mma && (M <= 8 || (M <= 16 && (N + tb200::kTc3TileW - 1) / tb200::kTc3TileW > sm_count() / 2)))
+        return TERNIX_B200_KERNEL_DECODE_MMA;
+    return gemm_tc_ok(dA, dW, K, N) ? TERNIX_B200_KERNEL_GEMM_TC : TERNIX_B200_KERNEL_GENERIC;
 }
 
 // Operands that the TMA unit cannot describe (ragged pitch or unaligned base), product too large for the generic kernel:
@@ -1282,7 +1333,7 @@ int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K,
     if (const int rc = host_call_pool(&pool)) return rc;
     // whether an aligned base and aligned pitches suffice for this kernel is what the pretended sizes ask
     const int Kp = static_cast<int>(a_pitch), Np = static_cast<int>(w_pitch * 4);
-    const int kernel = select_kernel(nullptr, nullptr, M, Kp, Np);
+    const int kernel = select_fused(nullptr, nullptr, M, Kp, Np);
     const bool copy_a = kernel != TERNIX_B200_KERNEL_GEMV && (K % 16 != 0 || !aligned(dA, 16));
     const bool copy_w = N % 64 != 0 || !aligned(dW, 16);
     const size_t a_bytes = copy_a ? static_cast<size_t>(M) * a_pitch : 0, w_bytes = copy_w ? static_cast<size_t>(K) * w_pitch : 0;
@@ -1320,13 +1371,13 @@ int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, 
     switch (kernel) {
         case TERNIX_B200_KERNEL_GEMV: if (!gemv_ok(dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
         case TERNIX_B200_KERNEL_DECODE_MMA: if (!decode_mma_ok(dA, dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
-        case TERNIX_B200_KERNEL_SKINNY_TC: if (!skinny_ok(dA, dW, M, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
+        case TERNIX_B200_KERNEL_SKINNY_TC: return TERNIX_B200_ERR_UNSUPPORTED;
         case TERNIX_B200_KERNEL_GEMM_TC: if (!gemm_tc_ok(dA, dW, K, N)) return TERNIX_B200_ERR_UNSUPPORTED; break;
         default: break;
     }
     if (K == 0) kernel = TERNIX_B200_KERNEL_GENERIC;           // empty sums: only the epilogue is left
     if (kernel == TERNIX_B200_KERNEL_AUTO) {
-        kernel = select_kernel(dA, dW, M, K, N);
+        kernel = select_fused(dA, dW, M, K, N);
         if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 &&
             (static_cast<double>(M) * K * N >= 3e7 || K >= 512))
             return launch_fused_aligned_copy(dA, dW, M, K, N, epi, d_status, st);

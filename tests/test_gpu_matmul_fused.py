@@ -100,7 +100,7 @@ def test_kernels_give_the_same_bits(shape, dtype, act):
     wide_r = torch.randn(M, N + 7, device="cuda").to(t)
     want = None
     for kernel in ("auto", "generic", "gemv", "decode_mma", "skinny_tc", "gemm_tc"):
-        if kernel == "gemv" and M > 16 or kernel == "skinny_tc" and M > 128:
+        if kernel == "gemv" and M > 16 or kernel == "skinny_tc":           # the latter has no fused form
             with pytest.raises(ValueError):
                 tb.matmul_fused(ta, tw, trs, tcs, kernel=kernel)
             continue

@@ -65,7 +65,7 @@ def test_glu_quantize_arguments(kw, code):
     (dict(w=None), tb.ERR_INVALID_ARG), (dict(y=None), tb.ERR_INVALID_ARG), (dict(y=P + 1), tb.ERR_INVALID_ARG),
     (dict(dt=0, y=P + 2), tb.ERR_INVALID_ARG), (dict(res=P + 1, ldr=64), tb.ERR_INVALID_ARG), (dict(rs=P + 1), tb.ERR_INVALID_ARG),
     (dict(cs=P + 2), tb.ERR_INVALID_ARG), (dict(kernel=tb.KERNEL_GEMV, M=17), tb.ERR_UNSUPPORTED),
-    (dict(kernel=tb.KERNEL_SKINNY_TC, M=129), tb.ERR_UNSUPPORTED), (dict(kernel=tb.KERNEL_DECODE_MMA, K=65), tb.ERR_UNSUPPORTED),
+    (dict(kernel=tb.KERNEL_SKINNY_TC), tb.ERR_UNSUPPORTED), (dict(kernel=tb.KERNEL_DECODE_MMA, K=65), tb.ERR_UNSUPPORTED),
     (dict(kernel=tb.KERNEL_GEMM_TC, N=68, ldy=68), tb.ERR_UNSUPPORTED), (dict(kernel=tb.KERNEL_GEMM_TC, a=P + 1), tb.ERR_UNSUPPORTED),
     (dict(M=0), tb.OK), (dict(N=0), tb.OK),
 ])
