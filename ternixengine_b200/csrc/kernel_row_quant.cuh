@@ -13,12 +13,15 @@
 // the NaN-propagating instruction and carried between lanes as bits (|NaN| > inf > any finite as integers).
 // 127 / m would overflow for m below 2^-121; such rows are scaled up by 2^100 first, which is exact.
 //
-// One CTA per row, the row spread over its threads as VPT vectors of 16 bytes each.
+// A row belongs to one CTA, spread over its threads as VPT vectors of 16 bytes each (or as single elements, where rows
+// start or end off a 16-byte boundary).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 #include "epilogue.cuh"
+#include "ptx_sm100.cuh"
 
 namespace tb200 {
 
@@ -54,6 +57,47 @@ union RowRaw {
         else *reinterpret_cast<uint4*>(p) = u;
     }
 };
+// The V elements as fp32; a bfloat16 is the upper half of its float: one instruction each.
+template <typename T, int V>
+__device__ __forceinline__ void row_unpack(const RowRaw<T, V>& x, float (&v)[V]) {
+    if constexpr (V == 8 && std::is_same_v<T, __nv_bfloat16>) {
+        const uint32_t w[4] = {x.u.x, x.u.y, x.u.z, x.u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else if constexpr (V == 8) {
+        const uint32_t w[4] = {x.u.x, x.u.y, x.u.z, x.u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = to_float<T>(x.t[i]);
+    }
+}
+// ... and back, rounded to T.
+template <typename T, int V>
+__device__ __forceinline__ void row_pack(RowRaw<T, V>& x, const float (&v)[V]) {
+    if constexpr (V == 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>)
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+            else
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+        }
+        x.u = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x.t[i] = from_float<T>(v[i]);
+    }
+}
 template <typename T, int V>
 __device__ __forceinline__ void row_load_weight(const void* w, int w_is_f32, int k, float (&v)[V]) {
     if constexpr (V == 1) {
@@ -67,30 +111,37 @@ __device__ __forceinline__ void row_load_weight(const void* w, int w_is_f32, int
                 v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
             }
         } else {
-            union { uint4 u; T t[V]; } x;
+            RowRaw<T, V> x;
             x.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w) + k));
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = to_float<T>(x.t[i]);
+            row_unpack<T, V>(x, v);
         }
     }
 }
-// V elements of a row from column k, loaded as x and y: what is normalised and quantised (h or z).  Writes h on the way.
-template <typename T, int MODE, int V>
-__device__ __forceinline__ void row_element(const RowQuantArgs& p, int row, int k, RowRaw<T, V>& x, const RowRaw<T, V>& y,
-                                            float (&v)[V]) {
+// A thread's part of a row, loaded as x and y, as what is normalised and quantised (h or z); h is written on the way.
+// `have`: how many of its VPT vectors lie inside the row; the others are zero and stay zero under every activation.
+template <typename T, int MODE, int VPT, int V>
+__device__ __forceinline__ void row_values(const RowQuantArgs& p, int row, int have, RowRaw<T, V> (&x)[VPT],
+                                           const RowRaw<T, V> (&y)[VPT], float (&t)[VPT][V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_float<T>(x.t[i]);
-    if constexpr (MODE == kRowNormResidual) {
+    for (int j = 0; j < VPT; ++j) row_unpack<T, V>(x[j], t[j]);
+    if constexpr (MODE == kRowGate) activate(p.act, reinterpret_cast<float (&)[VPT * V]>(t));       // one choice for all of them
+    if constexpr (MODE != kRowNorm) {
+        T* h = MODE == kRowNormResidual ? static_cast<T*>(p.h) + static_cast<size_t>(row) * p.ldh + threadIdx.x * V : nullptr;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            x.t[i] = from_float<T>(__fadd_rn(v[i], to_float<T>(y.t[i])));
-            v[i] = to_float<T>(x.t[i]);
+        for (int j = 0; j < VPT; ++j) {
+            float o[V];
+            row_unpack<T, V>(y[j], o);
+            if constexpr (MODE == kRowNormResidual) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) t[j][i] = __fadd_rn(t[j][i], o[i]);
+                row_pack<T, V>(x[j], t[j]);
+                row_unpack<T, V>(x[j], t[j]);
+                if (j < have) x[j].store(h + j * blockDim.x * V);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], o[i]);
+            }
         }
-        x.store(static_cast<T*>(p.h) + static_cast<size_t>(row) * p.ldh + k);
-    } else if constexpr (MODE == kRowGate) {
-        activate(p.act, v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = __fmul_rn(v[i], to_float<T>(y.t[i]));
     }
 }
 // Codes as the low bytes of t * inv + 1.5 * 2^23: the addition rounds to the nearest integer, ties to even, and leaves
@@ -119,106 +170,181 @@ __device__ __forceinline__ void row_reduce(uint32_t& top, float& sum, uint2 (*sl
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
 }
 
-// What the statistics of a row say about its codes.
+// What the statistics of a row say about its codes: q = rint((t * lift) * inv), all zero where keep is 0.
 struct RowScale {
-    float lift, inv, scale;    // q = rint((t * lift) * inv)
-    uint32_t keep;             // 0: the row's codes are all zero
+    float lift, inv;
+    uint32_t keep;
 };
 __device__ __forceinline__ RowScale row_scale_of(uint32_t top, float sum, const RowQuantArgs& p) {
-    RowScale r{1.0f, 0.0f, 1.0f, 0xffffffffu};
+    RowScale r{1.0f, 0.0f, 0xffffffffu};
     const float m = __uint_as_float(top);
-    const bool normed = p.eps >= 0.0f;
-    if (top >= 0x7f800000u || (normed && !(sum < __uint_as_float(0x7f800000u)))) {
-        r.scale = __uint_as_float(0x7fc00000u);
+    if (top >= 0x7f800000u || (p.eps >= 0.0f && !(sum < __uint_as_float(0x7f800000u)))) {
         r.keep = 0;
     } else if (m > 0.0f) {
         if (m < 1e-30f) r.lift = 1.2676506e30f;        // 2^100
-        const float top_l = __fmul_rn(m, r.lift);
-        r.inv = __fdiv_rn(127.0f, top_l);
-        r.scale = __fdiv_rn(top_l, 127.0f);
-        if (normed) r.scale = __fmul_rn(r.scale, __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.K)), p.eps))));
-        if (r.lift != 1.0f) r.scale = __fmul_rn(r.scale, 7.8886091e-31f);      // 2^-100: the one rounding to a subnormal
+        r.inv = __fdiv_rn(127.0f, __fmul_rn(m, r.lift));
     }
     return r;
 }
+// The row's scale: three divisions and a root, a hundred instructions, for one thread of the CTA only.
+__device__ __forceinline__ void row_store_scale(const RowQuantArgs& p, int row, uint32_t top, float sum, const RowScale& r) {
+    float scale = 1.0f;
+    if (!r.keep) {
+        scale = __uint_as_float(0x7fc00000u);
+    } else if (top) {
+        scale = __fdiv_rn(__fmul_rn(__uint_as_float(top), r.lift), 127.0f);
+        if (p.eps >= 0.0f) scale = __fmul_rn(scale, __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(sum, static_cast<float>(p.K)), p.eps))));
+        if (r.lift != 1.0f) scale = __fmul_rn(scale, 7.8886091e-31f);      // 2^-100: the one rounding to a subnormal
+    }
+    p.row_scale[row] = scale;
+}
 
+// One row, held in registers as t: statistics, scale, codes.  `slots` and `turn` as in row_reduce().
+template <typename T, int VPT, int V>
+__device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int have, float (&t)[VPT][V], uint2 (*slots)[32], int turn) {
+    const int w_is_f32 = p.w_dtype == kDtypeF32;
+    float top_f = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int k = (threadIdx.x + j * blockDim.x) * V;
+        if (p.eps >= 0.0f) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum = fmaf(t[j][i], t[j][i], sum);
+        }
+        if (p.w && j < have) {
+            float w[V];
+            row_load_weight<T, V>(p.w, w_is_f32, k, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) top_f = max_nan(top_f, fabsf(t[j][i]));
+    }
+    uint32_t top = __float_as_uint(top_f);
+    row_reduce(top, sum, slots, turn);
+    const RowScale r = row_scale_of(top, sum, p);
+    if (threadIdx.x == 0) row_store_scale(p, row, top, sum, r);
+    int8_t* q = p.q + static_cast<size_t>(row) * p.K + threadIdx.x * V;
+    if (r.lift != 1.0f) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[j][i] *= r.lift;
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        if (j >= have) continue;
+        int8_t* at = q + j * blockDim.x * V;
+        if constexpr (V == 1) {
+            *at = static_cast<int8_t>(row_code(t[j][0], r.inv) & r.keep);
+        } else {
+            uint32_t c[V / 4];
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i)
+                c[i] = pack_codes(row_code(t[j][4 * i], r.inv), row_code(t[j][4 * i + 1], r.inv),
+                                  row_code(t[j][4 * i + 2], r.inv), row_code(t[j][4 * i + 3], r.inv)) & r.keep;
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(c[0], c[1]);
+            else *reinterpret_cast<uint32_t*>(at) = c[0];
+        }
+    }
+}
+// Vectors of a row that fall to this thread: threadIdx.x, threadIdx.x + blockDim.x, ... below K / V.
+template <int V>
+__device__ __forceinline__ int row_have(int K) {
+    const int left = K / V - static_cast<int>(threadIdx.x);
+    return left <= 0 ? 0 : (left + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
+}
+
+// One row per CTA.
 template <typename T, int MODE, int VPT, bool kVec>
 __global__ void __launch_bounds__(1024)
 row_quant_kernel(const __grid_constant__ RowQuantArgs p) {
     constexpr int V = kVec ? kRowVec<T> : 1;
     __shared__ uint2 slots[2][32];
-    const int w_is_f32 = p.w_dtype == kDtypeF32;
+    const int row = blockIdx.x, have = row_have<V>(p.K);
+    float t[VPT][V];
+    // all of the row's loads first: a store of h between them would hold the next ones back (h may be x or y)
+    RowRaw<T, V> x[VPT], y[VPT];
+    const T* px = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx + threadIdx.x * V;
+    const T* py = MODE == kRowNorm ? nullptr : static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy + threadIdx.x * V;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        x[j].u = y[j].u = make_uint4(0, 0, 0, 0);
+        if (j < have) {
+            x[j].load(px + j * blockDim.x * V);
+            if constexpr (MODE != kRowNorm) y[j].load(py + j * blockDim.x * V);
+        }
+    }
+    row_values<T, MODE, VPT, V>(p, row, have, x, y, t);
+    row_finish<T, VPT, V>(p, row, have, t, slots, 0);
+}
+
+// Many rows: persistent CTAs that have the next row under way while they reduce and quantise this one.  A thread copies
+// its own vectors of the next row into shared memory with cp.async and reads only what it copied itself, so the copies
+// need no barrier; its slots are free as soon as this row's values are in registers.  (Without this an SM that holds one
+// row of 28672 in its registers has no load in flight from the reduction to the last store: 158 us against 106 us for 4096 rows.)
+template <typename T, int MODE, int VPT>
+__global__ void __launch_bounds__(VPT == 2 ? 512 : 1024, VPT == 2 ? 3 : 1)
+row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
+    constexpr int V = kRowVec<T>;
+    constexpr int kIn = MODE == kRowNorm ? 1 : 2;
+    extern __shared__ __align__(16) uint4 row_stage[];             // [VPT][kIn][threads]
+    __shared__ uint2 slots[2][32];
+    const uint32_t mine = smem_u32(row_stage) + threadIdx.x * 16, step = blockDim.x * 16;
+    const int have = row_have<V>(p.K);
+    const size_t stride = static_cast<size_t>(blockDim.x) * 16;              // bytes between a thread's vectors
+    auto fetch = [&](const char* x, const char* y, int j) {
+        if (j >= have) return;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (j * kIn) * step), "l"(x + j * stride) : "memory");
+        if constexpr (MODE != kRowNorm)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (j * kIn + 1) * step), "l"(y + j * stride) : "memory");
+    };
+    auto row_x = [&](int row) { return static_cast<const char*>(p.x) + (static_cast<size_t>(row) * p.ldx + threadIdx.x * V) * sizeof(T); };
+    auto row_y = [&](int row) {
+        return MODE == kRowNorm ? nullptr : static_cast<const char*>(p.y) + (static_cast<size_t>(row) * p.ldy + threadIdx.x * V) * sizeof(T);
+    };
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        fetch(row_x(blockIdx.x), row_y(blockIdx.x), j);
+        if (j >= have) {             // slots that no copy writes are read as zero
+            sts_v4(mine + (j * kIn) * step, make_uint4(0, 0, 0, 0));
+            if constexpr (kIn == 2) sts_v4(mine + (j * kIn + 1) * step, make_uint4(0, 0, 0, 0));
+        }
+    }
     int turn = 0;
     for (int row = blockIdx.x; row < p.M; row += gridDim.x, turn ^= 1) {
         float t[VPT][V];
-        float top_f = 0.0f, sum = 0.0f;
-        // all of the row's loads first: a store of h between them would hold the next ones back (h may be x or y)
         RowRaw<T, V> x[VPT], y[VPT];
+        const int next = row + static_cast<int>(gridDim.x);
+        const char *nx = row_x(next), *ny = row_y(next);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // Each vector's slots are requested again as soon as they have been read (a thread's shared-memory accesses are
+        // performed in order, and nobody else touches its slots), before any arithmetic on this row.
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int k = (threadIdx.x + j * blockDim.x) * V;
-            x[j].u = y[j].u = make_uint4(0, 0, 0, 0);
-            if (k < p.K) {
-                x[j].load(static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx + k);
-                if constexpr (MODE != kRowNorm) y[j].load(static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy + k);
-            }
+            x[j].u = lds_v4(mine + (j * kIn) * step);
+            y[j].u = kIn == 2 ? lds_v4(mine + (j * kIn + 1) * step) : make_uint4(0, 0, 0, 0);
+            if (next < p.M) fetch(nx, ny, j);
         }
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int k = (threadIdx.x + j * blockDim.x) * V;
-            if (k < p.K) {
-                row_element<T, MODE, V>(p, row, k, x[j], y[j], t[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) t[j][i] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int k = (threadIdx.x + j * blockDim.x) * V;
-#pragma unroll
-            for (int i = 0; i < V; ++i) sum = fmaf(t[j][i], t[j][i], sum);
-            if (p.w && k < p.K) {
-                float w[V];
-                row_load_weight<T, V>(p.w, w_is_f32, k, w);
-#pragma unroll
-                for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], w[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) top_f = max_nan(top_f, fabsf(t[j][i]));
-        }
-        uint32_t top = __float_as_uint(top_f);
-        row_reduce(top, sum, slots, turn);
-        const RowScale r = row_scale_of(top, sum, p);
-        if (threadIdx.x == 0) p.row_scale[row] = r.scale;
-        int8_t* q = p.q + static_cast<size_t>(row) * p.K;
-        if (r.lift != 1.0f) {
-#pragma unroll
-            for (int j = 0; j < VPT; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) t[j][i] *= r.lift;
-        }
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int k = (threadIdx.x + j * blockDim.x) * V;
-            if (k >= p.K) continue;
-            if constexpr (V == 1) {
-                q[k] = static_cast<int8_t>(row_code(t[j][0], r.inv) & r.keep);
-            } else {
-                uint32_t c[V / 4];
-#pragma unroll
-                for (int i = 0; i < V / 4; ++i)
-                    c[i] = pack_codes(row_code(t[j][4 * i], r.inv), row_code(t[j][4 * i + 1], r.inv),
-                                      row_code(t[j][4 * i + 2], r.inv), row_code(t[j][4 * i + 3], r.inv)) & r.keep;
-                if constexpr (V == 8) *reinterpret_cast<uint2*>(q + k) = make_uint2(c[0], c[1]);
-                else *reinterpret_cast<uint32_t*>(q + k) = c[0];
-            }
-        }
+        row_values<T, MODE, VPT, V>(p, row, have, x, y, t);
+        row_finish<T, VPT, V>(p, row, have, t, slots, turn);
     }
 }
 
 // Rows that do not fit the registers of a CTA: the same arithmetic, with the row computed twice.  The second pass reads
 // h back instead of adding again (it may have replaced the residual).
+template <typename T, int MODE>
+__device__ __forceinline__ void row_single(const RowQuantArgs& p, int row, int k, RowRaw<T, 1>& x, const RowRaw<T, 1>& y, float (&t)[1]) {
+    t[0] = to_float<T>(x.t[0]);
+    if constexpr (MODE == kRowNormResidual) {
+        x.t[0] = from_float<T>(__fadd_rn(t[0], to_float<T>(y.t[0])));
+        t[0] = to_float<T>(x.t[0]);
+        x.store(static_cast<T*>(p.h) + static_cast<size_t>(row) * p.ldh + k);
+    } else if constexpr (MODE == kRowGate) {
+        activate(p.act, t);
+        t[0] = __fmul_rn(t[0], to_float<T>(y.t[0]));
+    }
+}
 template <typename T, int MODE>
 __global__ void __launch_bounds__(1024)
 row_quant_long_kernel(const __grid_constant__ RowQuantArgs p) {
@@ -232,7 +358,7 @@ row_quant_long_kernel(const __grid_constant__ RowQuantArgs p) {
             float t[1];
             x.load(static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx + k);
             if constexpr (MODE != kRowNorm) y.load(static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy + k);
-            row_element<T, MODE, 1>(p, row, k, x, y, t);
+            row_single<T, MODE>(p, row, k, x, y, t);
             sum = fmaf(t[0], t[0], sum);
             if (p.w) {
                 float w[1];
@@ -244,7 +370,7 @@ row_quant_long_kernel(const __grid_constant__ RowQuantArgs p) {
         uint32_t top = __float_as_uint(top_f);
         row_reduce(top, sum, slots, turn);
         const RowScale r = row_scale_of(top, sum, p);
-        if (threadIdx.x == 0) p.row_scale[row] = r.scale;
+        if (threadIdx.x == 0) row_store_scale(p, row, top, sum, r);
         int8_t* q = p.q + static_cast<size_t>(row) * p.K;
         for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
             RowRaw<T, 1> x, y;
@@ -254,7 +380,7 @@ row_quant_long_kernel(const __grid_constant__ RowQuantArgs p) {
             } else {
                 x.load(static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx + k);
                 if constexpr (MODE == kRowGate) y.load(static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy + k);
-                row_element<T, MODE, 1>(p, row, k, x, y, t);
+                row_single<T, MODE>(p, row, k, x, y, t);
             }
             if (p.w) {
                 float w[1];

@@ -1155,6 +1155,26 @@ int launch_row_quant_t(const tb200::RowQuantArgs& p, int threads, cudaStream_t s
     TB_CUDA(cudaGetLastError());
     return TERNIX_B200_OK;
 }
+constexpr size_t kRowStreamSmem = 200 * 1024;
+template <typename T, int MODE, int VPT>
+int launch_row_quant_stream_t(const tb200::RowQuantArgs& p, int threads, cudaStream_t st) {
+    constexpr auto kern = tb200::row_quant_stream_kernel<T, MODE, VPT>;
+    if (const int rc = ensure_smem_attr<kern>(kRowStreamSmem)) return rc;
+    const size_t smem = static_cast<size_t>(VPT) * (MODE == tb200::kRowNorm ? 1 : 2) * threads * 16;
+    // what an SM holds, asked once per device and thread count
+    static std::atomic<int> cache[kMaxDevices][33] = {};
+    std::atomic<int>& slot = cache[current_device()][threads / 32];
+    int per_sm = slot.load(std::memory_order_relaxed);
+    if (per_sm <= 0) {
+        TB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem));
+        per_sm = std::max(1, per_sm);
+        slot.store(per_sm, std::memory_order_relaxed);
+    }
+    const int grid = std::min(p.M, per_sm * sm_count());
+    kern<<<grid, threads, smem, st>>>(p);
+    TB_CUDA(cudaGetLastError());
+    return TERNIX_B200_OK;
+}
 
 template <typename T, int MODE>
 int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
@@ -1165,6 +1185,19 @@ int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
     auto threads_for = [&](int items, int vpt) { return std::max(32, ((items + vpt - 1) / vpt + 31) / 32 * 32); };
     if (vec) {
         const int items = p.K / V;
+        // Rows of more than 8 KB an operand, enough of them to come in rounds: persistent CTAs with the next row under way
+        // (4096 x 8192 bfloat16 with residual 42 us against 49, 4096 x 28672 gate 88 against 119; below that size an SM holds
+        // many rows at once and nothing is gained: 4096 x 2560 16.7 us either way).  float32 with a residual moves so many
+        // bytes a row that it runs at the copy rate without (4096 x 8192: 68 us against 80).
+        constexpr bool kStream = !(sizeof(T) == 4 && MODE == tb200::kRowNormResidual);
+        if constexpr (kStream) {
+            if (items > 512 && p.M >= 2 * sm_count()) {
+                if (MODE != tb200::kRowGate && items <= 1024) return launch_row_quant_stream_t<T, MODE, 2>(p, threads_for(items, 2), st);
+                const int threads = threads_for(items, 4);
+                if (items <= 4096 && static_cast<size_t>(MODE == tb200::kRowNorm ? 64 : 128) * threads <= kRowStreamSmem)
+                    return launch_row_quant_stream_t<T, MODE, 4>(p, threads, st);
+            }
+        }
         if (items <= 512) return launch_row_quant_t<T, MODE, 1, true>(p, threads_for(items, 1), st);
         if (items <= 1024) return launch_row_quant_t<T, MODE, 2, true>(p, threads_for(items, 2), st);
         if (items <= 4096) return launch_row_quant_t<T, MODE, 4, true>(p, threads_for(items, 4), st);
