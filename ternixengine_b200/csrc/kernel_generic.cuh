@@ -150,8 +150,9 @@ ternary_generic_fused_kernel(const int8_t* __restrict__ A, const uint8_t* __rest
             }
         }
         __syncthreads();
+        const int groups = row0 + ty * 4 < M ? kGenK / 4 : 0;        // a warp without rows only helps to stage
 #pragma unroll 4
-        for (int g = 0; g < kGenK / 4; ++g) {
+        for (int g = 0; g < groups; ++g) {
             const uint32_t t = sW[g][tx];
             int a4[4];
 #pragma unroll
@@ -186,20 +187,27 @@ ternary_generic_fused_kernel(const int8_t* __restrict__ A, const uint8_t* __rest
     }
 }
 
-// Rows of `width` bytes at any address and pitch, copied to rows at a pitch (and base) of 16 bytes, which is what the TMA
-// unit can describe.  A thread writes 16 bytes and reads them as aligned words; a word that is not wholly inside the
-// source is put together from its bytes.  What lies between the width and the pitch is zeroed.
+// Rows of `width` bytes at any address, copied to rows at a pitch (and base) of 16 bytes, which is what the TMA unit can
+// describe.  A thread writes 16 bytes and reads them as aligned words; a word that is not wholly inside the source is put
+// together from its bytes.  What lies between the width and the pitch is zeroed.  One launch copies both operands of a
+// product: the first a.blocks CTAs the one, the others the other.
+struct AlignJob {
+    const uint8_t* src;      // [rows][width], no gaps
+    uint8_t* dst;            // [rows][pitch]
+    long long rows;
+    int width, pitch, blocks;
+};
 __global__ void __launch_bounds__(256)
-align_rows_kernel(const uint8_t* __restrict__ src, long long src_pitch, uint8_t* __restrict__ dst, int dst_pitch, int width,
-                  long long rows) {
-    const int per_row = dst_pitch / 16;
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(src);
-    const uintptr_t hi = lo + static_cast<uintptr_t>(rows - 1) * src_pitch + width;
-    const long long total = rows * per_row;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
+align_rows_kernel(const __grid_constant__ AlignJob a, const __grid_constant__ AlignJob b) {
+    const bool first = static_cast<int>(blockIdx.x) < a.blocks;
+    const AlignJob& job = first ? a : b;
+    const int per_row = job.pitch / 16, width = job.width;
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(job.src), hi = lo + static_cast<uintptr_t>(job.rows) * width;
+    const long long total = job.rows * per_row, block = first ? blockIdx.x : blockIdx.x - a.blocks;
+    for (long long i = block * 256 + threadIdx.x; i < total; i += job.blocks * 256LL) {
         const long long r = i / per_row;
         const int x = static_cast<int>(i - r * per_row) * 16;
-        const uintptr_t at = lo + static_cast<uintptr_t>(r) * src_pitch + x, word = at & ~uintptr_t(3);
+        const uintptr_t at = lo + static_cast<uintptr_t>(r) * width + x, word = at & ~uintptr_t(3);
         const int shift = static_cast<int>(at & 3) * 8;
         uint32_t w[5];
 #pragma unroll
@@ -211,8 +219,8 @@ align_rows_kernel(const uint8_t* __restrict__ src, long long src_pitch, uint8_t*
                 w[j] = __ldg(reinterpret_cast<const uint32_t*>(p));
             } else {
 #pragma unroll
-                for (int b = 0; b < 4; ++b)
-                    if (p + b >= lo && p + b < hi) w[j] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(p + b)) << (8 * b);
+                for (int c = 0; c < 4; ++c)
+                    if (p + c >= lo && p + c < hi) w[j] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t*>(p + c)) << (8 * c);
             }
         }
         uint32_t o[4];
@@ -222,7 +230,7 @@ align_rows_kernel(const uint8_t* __restrict__ src, long long src_pitch, uint8_t*
             const int left = width - x - 4 * j;             // bytes of this word that belong to the row
             if (left < 4) o[j] &= left <= 0 ? 0u : (1u << (8 * left)) - 1u;
         }
-        *reinterpret_cast<uint4*>(dst + r * dst_pitch + x) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(job.dst + r * job.pitch + x) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 

@@ -1372,27 +1372,27 @@ int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K,
     const size_t a_bytes = copy_a ? static_cast<size_t>(M) * a_pitch : 0, w_bytes = copy_w ? static_cast<size_t>(K) * w_pitch : 0;
     uint8_t* tmp = nullptr;
     TB_CUDA(cudaMallocFromPoolAsync(reinterpret_cast<void**>(&tmp), (a_bytes + 255) / 256 * 256 + w_bytes, pool, st));
-    auto copy = [&](const void* src, long long src_pitch, uint8_t* dst, long long pitch, int width, long long rows) {
+    auto job = [&](const void* src, uint8_t* dst, long long rows, int width, long long pitch) {
         const long long blocks = std::min<long long>((rows * (pitch / 16) + 255) / 256, 8LL * sm_count());
-        tb200::align_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const uint8_t*>(src), src_pitch, dst,
-                                                                                static_cast<int>(pitch), width, rows);
-        return cudaGetLastError();
+        return tb200::AlignJob{static_cast<const uint8_t*>(src), dst, rows, width, static_cast<int>(pitch), static_cast<int>(blocks)};
     };
     Pitches pt;
     const int8_t* a = dA;
     const uint8_t* w = dW;
-    cudaError_t e = cudaSuccess;
+    tb200::AlignJob ja{}, jw{};
     if (copy_a) {
-        e = copy(dA, K, tmp, a_pitch, K, M);
+        ja = job(dA, tmp, M, K, a_pitch);
         a = reinterpret_cast<const int8_t*>(tmp);
         pt.a = a_pitch;
     }
-    if (copy_w && e == cudaSuccess) {
+    if (copy_w) {
         uint8_t* dst = tmp + (a_bytes + 255) / 256 * 256;
-        e = copy(dW, N / 4, dst, w_pitch, N / 4, K);
+        jw = job(dW, dst, K, N / 4, w_pitch);
         w = dst;
         pt.w = w_pitch;
     }
+    tb200::align_rows_kernel<<<static_cast<unsigned>(ja.blocks + jw.blocks), 256, 0, st>>>(ja, jw);
+    const cudaError_t e = cudaGetLastError();
     const int rc = e != cudaSuccess ? cuda_fail(e) : launch_fused_tma(kernel, a, w, M, K, N, pt, epi, d_status, st);
     cudaFreeAsync(tmp, st);
     return rc;
@@ -1411,8 +1411,11 @@ int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, 
     if (K == 0) kernel = TERNIX_B200_KERNEL_GENERIC;           // empty sums: only the epilogue is left
     if (kernel == TERNIX_B200_KERNEL_AUTO) {
         kernel = select_fused(dA, dW, M, K, N);
-        if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 &&
-            (static_cast<double>(M) * K * N >= 3e7 || K >= 512))
+        // The generic kernel takes 1.5 us per 64 k-rows and round of tiles; an aligned copy and the kernel behind it from
+        // 6 (1 x 1000 x 4004: 6.1 against 26 us) to 10 us (129 x 1029 x 2052: 10 against 31; 1024 x 100 x 1028: 11.4 against 7.6).
+        const double slabs = (K + tb200::kGenK - 1) / tb200::kGenK;
+        const double tiles = static_cast<double>((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes) * ((M + tb200::kGenRows - 1) / tb200::kGenRows);
+        if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 && slabs * std::max(1.0, tiles / sm_count()) > 4)
             return launch_fused_aligned_copy(dA, dW, M, K, N, epi, d_status, st);
     }
     if (kernel != TERNIX_B200_KERNEL_GENERIC) return launch_fused_tma(kernel, dA, dW, M, K, N, Pitches{}, epi, d_status, st);
