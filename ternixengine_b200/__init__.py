@@ -433,6 +433,7 @@ class _Runtime:
         self.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
         self.f32, self.i8, self.u8, self.bf16 = torch.float32, torch.int8, torch.uint8, torch.bfloat16
         self.empty, self.Tensor, self.guard = torch.empty, torch.Tensor, torch.cuda.device
+        self.scale_types = (torch.float32,)
         self.current_device, self.raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
@@ -450,8 +451,10 @@ def _rows(t, name, dev, dtype, shape) -> int:
     """Checks a row-major operand with unit column stride and returns its row pitch in elements."""
     if t.dtype is not dtype or t.get_device() != dev or t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype} on cuda:{dev}")
-    ld, inner = t.stride()
     M, K = shape
+    if t.is_contiguous():
+        return K
+    ld, inner = t.stride()
     if inner != 1 and K > 1:
         raise ValueError(f"{name} must have unit column stride")
     if M <= 1:
@@ -463,7 +466,7 @@ def _rows(t, name, dev, dtype, shape) -> int:
 
 def _vector(t, name, dev, dtypes, n) -> int:
     """Checks a contiguous vector and returns its address."""
-    if t.dtype not in dtypes or t.get_device() != dev or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.dtype not in dtypes or t.get_device() != dev or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be ({n},) of {' or '.join(str(d) for d in dtypes)} on cuda:{dev}, contiguous")
     return t.data_ptr()
 
@@ -475,7 +478,7 @@ def _quantized_out(rt, dev, shape, out, row_scale):
         raise ValueError(f"out must be a contiguous {tuple(shape)} int8 tensor on cuda:{dev}")
     if row_scale is None:
         row_scale = rt.empty(shape[0], dtype=rt.f32, device=f"cuda:{dev}")
-    return out, row_scale, _vector(row_scale, "row_scale", dev, (rt.f32,), shape[0])
+    return out, row_scale, _vector(row_scale, "row_scale", dev, rt.scale_types, shape[0])
 
 
 def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None, row_scale=None, residual_out=None):
@@ -592,14 +595,14 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
     pc = pb = pr = None
     ws, b_dtype, ldr = 0.0, 0, 0
     if isinstance(w_scale, rt.Tensor):
-        pc = _vector(w_scale, "w_scale", dev, (rt.f32,), N)
+        pc = _vector(w_scale, "w_scale", dev, rt.scale_types, N)
     else:
         ws = w_scale
     if bias is not None:
         pb, b_dtype = _vector(bias, "bias", dev, rt.codes, N), rt.codes[bias.dtype]
     if residual is not None:
         pr, ldr = residual.data_ptr(), _rows(residual, "residual", dev, dtype, (M, N))
-    ep = _Epilogue(_vector(row_scale, "row_scale", dev, (rt.f32,), M), pc, ws, act, pb, b_dtype, code, pr, ldr)
+    ep = _Epilogue(_vector(row_scale, "row_scale", dev, rt.scale_types, M), pc, ws, act, pb, b_dtype, code, pr, ldr)
     args = (a.data_ptr(), w_packed.data_ptr(), ep, out.data_ptr(), ldy, M, K, N, kern,
             status.data_ptr() if status is not None else None, rt.raw_stream(dev))
     if rt.current_device() == dev:
