@@ -153,6 +153,7 @@ ternary_decode_mma_kernel(const __grid_constant__ MmaProblem single, const MmaSi
         mbar_init_fence();
     }
     __syncthreads();
+    if constexpr (Epi::kFused) dependent_wait();
 
     if (warp == kMmaConsumerWarps) {
         // ------------------------------------------------------------ producer lane

@@ -110,6 +110,7 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
     // The CTAs of the cluster meet here, but nobody waits for the others yet: loads and expansion touch this CTA only.  The
     // first thing that needs a peer is the arrival on the leader's `ready` barrier.
     cluster_arrive();
+    dependent_wait();
 
     if (warp == 0) {
         // ================================================================ activations

@@ -358,6 +358,7 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
+    if constexpr (Epi::kFused) dependent_wait();
 
     // Each role branch opens with its register hand-over, so that the compiler sees how many registers the code behind it may use.
     if (warp < kTc3FirstExpandWarp) {

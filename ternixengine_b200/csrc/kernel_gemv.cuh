@@ -85,6 +85,7 @@ ternary_gemv_kernel(const __grid_constant__ CUtensorMap tmap_w, const int8_t* __
     }
     for (int i = tid; i < MR * 16 * (WORDS + 1); i += kGemvThreads) part[i] = 0;
     __syncthreads();
+    if constexpr (Epi::kFused) dependent_wait();
 
     if (warp == kGemvConsumerWarps) {
         // ------------------------------------------------------------ producer: one lane drives TMA

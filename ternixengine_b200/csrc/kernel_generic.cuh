@@ -122,6 +122,7 @@ ternary_generic_fused_kernel(const int8_t* __restrict__ A, const uint8_t* __rest
     const int tid = threadIdx.x, tx = tid & 31, ty = tid >> 5;
     const int pitch = N >> 2;
     const int row0 = blockIdx.y * kGenRows, byte0 = blockIdx.x * kGenBytes;
+    dependent_wait();
 
     int32_t acc[4][4] = {}, total[4][4] = {};
     const int a_row = tid >> 3, a_k = (tid & 7) * 8;

@@ -262,6 +262,7 @@ row_quant_kernel(const __grid_constant__ RowQuantArgs p) {
     constexpr int V = kVec ? kRowVec<T> : 1;
     __shared__ uint2 slots[2][32];
     const int row = blockIdx.x, have = row_have<V>(p.K);
+    dependent_wait();
     float t[VPT][V];
     // all of the row's loads first: a store of h between them would hold the next ones back (h may be x or y)
     RowRaw<T, V> x[VPT], y[VPT];
@@ -303,6 +304,7 @@ row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
     auto row_y = [&](int row) {
         return MODE == kRowNorm ? nullptr : static_cast<const char*>(p.y) + (static_cast<size_t>(row) * p.ldy + threadIdx.x * V) * sizeof(T);
     };
+    dependent_wait();
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         fetch(row_x(blockIdx.x), row_y(blockIdx.x), j);
@@ -351,6 +353,7 @@ row_quant_long_kernel(const __grid_constant__ RowQuantArgs p) {
     __shared__ uint2 slots[2][32];
     const int w_is_f32 = p.w_dtype == kDtypeF32;
     int turn = 0;
+    dependent_wait();
     for (int row = blockIdx.x; row < p.M; row += gridDim.x, turn ^= 1) {
         float top_f = 0.0f, sum = 0.0f;
         for (int k = threadIdx.x; k < p.K; k += blockDim.x) {

@@ -203,6 +203,15 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t
     return d;
 }
 
+// ---------------------------------------------------------------- programmatic dependent launches
+// A kernel launched as a programmatic dependent may begin while the kernel before it still runs: dependent_wait() returns
+// when everything before it in the stream has completed and is visible.  Only then does it let the kernel after it begin,
+// so that whatever that one does before its own wait finds all work complete but this kernel's.
+__device__ __forceinline__ void dependent_wait() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- clusters / distributed smem
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;

@@ -15,6 +15,7 @@
 #include <mutex>
 #include <new>
 #include <queue>
+#include <utility>
 #include <vector>
 
 #include "kernel_gemm_tc.cuh"
@@ -167,6 +168,7 @@ struct Options {
     int skinny_group_lo = 17, skinny_group_hi = 128;   // the same for members of a problem group (one launch serves many products there)
     int skinny_split = 1;              // 0: never share a block between CTAs; 1: only when blocks outnumber SMs; 2: whenever it evens the load
     int split_rows = 0, split_cut = 0; // fused product: tile rows (64|128|256) and pairs per tile (1|2|4) of the cut prefill form; 0 = by shape
+    int layer_pdl = 1;                 // layer kernels as programmatic dependents of the kernel before them
     int host_slab = -1;                // slab extent of the pipelined host-pointer call; 0 = off, -1 = plan
     bool host_slab_rows = false;
 };
@@ -185,6 +187,7 @@ int apply_option(const char* name, const char* value) {
     else if (!std::strcmp(name, "gemv_pdl")) g_opt.gemv_pdl = num(def.gemv_pdl);
     else if (!std::strcmp(name, "mma_slices")) g_opt.mma_slices = num(def.mma_slices);
     else if (!std::strcmp(name, "mma_cluster")) g_opt.mma_cluster = num(def.mma_cluster);
+    else if (!std::strcmp(name, "layer_pdl")) g_opt.layer_pdl = num(def.layer_pdl) != 0;
     else if (!std::strcmp(name, "skinny_split")) g_opt.skinny_split = num(def.skinny_split);
     else if (!std::strcmp(name, "gemv_plan")) {
         g_opt.gemv_words = def.gemv_words; g_opt.gemv_split = def.gemv_split;
@@ -216,7 +219,7 @@ const Options& options() {
     static std::once_flag once;
     std::call_once(once, [] {
         static const char* const names[] = {"tc3", "tc_tile_rows", "tc_bn", "tc_ksplit", "gemv_plan", "group_words", "gemv_pdl", "mma_rows", "mma_slices",
-                                            "mma_cluster", "skinny_rows", "skinny_group_rows", "skinny_split", "fused_split", "host_slab"};
+                                            "mma_cluster", "skinny_rows", "skinny_group_rows", "skinny_split", "fused_split", "layer_pdl", "host_slab"};
         std::lock_guard<std::mutex> lock(g_opt_mutex);
         for (const char* n : names) {
             char env[64] = "TERNIX_B200_";
@@ -294,6 +297,27 @@ int select_kernel(const void* dA, const void* dW, int M, int K, int N) {
 }
 
 // ---------------------------------------------------------------- launches
+// Launches of the layer kernels (epilogue.cuh, kernel_row_quant.cuh): optional cluster along x, and as a programmatic
+// dependent of whatever comes before (every such kernel waits for it before its first access to global memory).
+template <typename... P, typename... A>
+int launch_layer(void (*kern)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, A&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = options().layer_pdl;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    TB_CUDA(cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...));
+    return TERNIX_B200_OK;
+}
 // Bytes between the rows of A and the k-rows of W where they are not K and N / 4 (copies made for the TMA unit); 0: as is.
 struct Pitches {
     long long a = 0, w = 0;
@@ -381,7 +405,9 @@ int launch_gemv_t(const CUtensorMap& tmap, const int8_t* dA, int32_t* dC, int M,
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const int a_words_ok = (K % 4 == 0) && aligned(dA, 4);
-    TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap, dA, dC, M, K, N, ldc, p.krange, a_words_ok, d_status, epi));
+    if constexpr (Epi::kFused)
+        return launch_layer(kern, cfg.gridDim, tb200::kGemvThreads, smem, p.ksplit, st, tmap, dA, dC, M, K, N, ldc, p.krange, a_words_ok, d_status, epi);
+    else TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap, dA, dC, M, K, N, ldc, p.krange, a_words_ok, d_status, epi));
     return TERNIX_B200_OK;
 }
 
@@ -501,7 +527,9 @@ int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M,
         const tb200::MmaProblem* no_probs = nullptr;
         const tb200::MmaItem* no_items = nullptr;
         const int* no_first = nullptr;
-        TB_CUDA(cudaLaunchKernelEx(&cfg, kern, prob, sg, no_probs, no_items, no_first, d_status, epi));
+        if constexpr (Epi::kFused)
+            return launch_layer(kern, cfg.gridDim, tb200::kMmaThreads, tb200::kMmaSmemBytes, cluster, st, prob, sg, no_probs, no_items, no_first, d_status, epi);
+        else TB_CUDA(cudaLaunchKernelEx(&cfg, kern, prob, sg, no_probs, no_items, no_first, d_status, epi));
         return TERNIX_B200_OK;
     }
     sg.tiles_per_slice = (sg.total_tiles + slices - 1) / slices;
@@ -509,6 +537,10 @@ int launch_decode_mma_t(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M,
     sg.add = sg.slices > 1;
     if (sg.add) TB_CUDA(cudaMemset2DAsync(dC, static_cast<size_t>(ldc) * 4, 0, static_cast<size_t>(N) * 4, M, st));
     const int grid = std::min(resident, base_items * sg.slices);
+    if constexpr (Epi::kFused)
+        return launch_layer(kern, dim3(static_cast<unsigned>(grid)), tb200::kMmaThreads, tb200::kMmaSmemBytes, 1, st, prob, sg,
+                            static_cast<const tb200::MmaProblem*>(nullptr), static_cast<const tb200::MmaItem*>(nullptr),
+                            static_cast<const int*>(nullptr), d_status, epi);
     kern<<<grid, tb200::kMmaThreads, tb200::kMmaSmemBytes, st>>>(prob, sg, nullptr, nullptr, nullptr, d_status, epi);
     TB_CUDA(cudaGetLastError());
     return TERNIX_B200_OK;
@@ -637,7 +669,11 @@ int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w,
     const tb200::Tc3Problem* no_probs = nullptr;
     const tb200::Tc2Tile* no_tiles = nullptr;
     const int* no_first = nullptr;
-    TB_CUDA(cudaLaunchKernelEx(&cfg, tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>, tmap_a, tmap_w, stores, dC0, M, K, N, ldc,
+    if constexpr (Epi::kFused)
+        return launch_layer(tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>, cfg.gridDim, tb200::kTc3Threads, smem, 2, st, tmap_a,
+                            tmap_w, stores, dC0, M, K, N, ldc, no_probs, no_tiles, no_first, d_status, static_cast<const float*>(nullptr),
+                            1.0f, epi);
+    else TB_CUDA(cudaLaunchKernelEx(&cfg, tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>, tmap_a, tmap_w, stores, dC0, M, K, N, ldc,
                                no_probs, no_tiles, no_first, d_status, static_cast<const float*>(nullptr), 1.0f, epi));
     return TERNIX_B200_OK;
 }
@@ -1151,9 +1187,7 @@ bool activation_ok(int a) { return a >= TERNIX_B200_ACT_NONE && a <= TERNIX_B200
 
 template <typename T, int MODE, int VPT, bool kVec>
 int launch_row_quant_t(const tb200::RowQuantArgs& p, int threads, cudaStream_t st) {
-    tb200::row_quant_kernel<T, MODE, VPT, kVec><<<p.M, threads, 0, st>>>(p);
-    TB_CUDA(cudaGetLastError());
-    return TERNIX_B200_OK;
+    return launch_layer(tb200::row_quant_kernel<T, MODE, VPT, kVec>, dim3(static_cast<unsigned>(p.M)), threads, 0, 1, st, p);
 }
 constexpr size_t kRowStreamSmem = 200 * 1024;
 template <typename T, int MODE, int VPT>
@@ -1171,9 +1205,7 @@ int launch_row_quant_stream_t(const tb200::RowQuantArgs& p, int threads, cudaStr
         slot.store(per_sm, std::memory_order_relaxed);
     }
     const int grid = std::min(p.M, per_sm * sm_count());
-    kern<<<grid, threads, smem, st>>>(p);
-    TB_CUDA(cudaGetLastError());
-    return TERNIX_B200_OK;
+    return launch_layer(kern, dim3(static_cast<unsigned>(grid)), threads, smem, 1, st, p);
 }
 
 template <typename T, int MODE>
@@ -1205,9 +1237,7 @@ int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
         if (p.K <= 4096) return launch_row_quant_t<T, MODE, 4, false>(p, threads_for(p.K, 4), st);
         if (p.K <= 16384) return launch_row_quant_t<T, MODE, 16, false>(p, threads_for(p.K, 16), st);
     }
-    tb200::row_quant_long_kernel<T, MODE><<<p.M, 1024, 0, st>>>(p);
-    TB_CUDA(cudaGetLastError());
-    return TERNIX_B200_OK;
+    return launch_layer(tb200::row_quant_long_kernel<T, MODE>, dim3(static_cast<unsigned>(p.M)), 1024, 0, 1, st, p);
 }
 
 template <int MODE>
@@ -1222,9 +1252,7 @@ template <typename Epi>
 int launch_generic_fused(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Epi& epi, cudaStream_t st) {
     dim3 grid((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes, (M + tb200::kGenRows - 1) / tb200::kGenRows);
     if (grid.y > 65535) return TERNIX_B200_ERR_INVALID_SHAPE;
-    tb200::ternary_generic_fused_kernel<<<grid, tb200::kGenThreads, 0, st>>>(dA, dW, M, K, N, epi);
-    TB_CUDA(cudaGetLastError());
-    return TERNIX_B200_OK;
+    return launch_layer(tb200::ternary_generic_fused_kernel<Epi>, grid, tb200::kGenThreads, 0, 1, st, dA, dW, M, K, N, epi);
 }
 
 // The cut prefill form (kernel_gemm_split.cuh): tile rows, and pairs that share a tile's K.
@@ -1237,20 +1265,8 @@ int launch_gemm_split_t(const int8_t* dA, const uint8_t* dW, int M, int K, int N
     if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, TA, pt.a)) return rc;
     if (const int rc = make_tc3_weight_map(&tmap_w, dW, K, N, pt.w)) return rc;
     const long tiles = static_cast<long>((M + TA - 1) / TA) * ((N + tb200::kTc3TileW - 1) / tb200::kTc3TileW);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * 2 * cut));
-    cfg.blockDim = dim3(tb200::kSpThreads);
-    cfg.dynamicSmemBytes = tb200::SpGeom<TA>::kSmemBytes;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(2 * cut);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    TB_CUDA(cudaLaunchKernelEx(&cfg, kern, tmap_a, tmap_w, M, K, N, cut, d_status, epi));
-    return TERNIX_B200_OK;
+    return launch_layer(kern, dim3(static_cast<unsigned>(tiles * 2 * cut)), tb200::kSpThreads, tb200::SpGeom<TA>::kSmemBytes, 2 * cut, st,
+                        tmap_a, tmap_w, M, K, N, cut, d_status, epi);
 }
 // Clusters of the cut form that the device holds at once (asked once per device and form).
 template <int TA, typename Epi>

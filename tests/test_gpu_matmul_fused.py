@@ -311,3 +311,84 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("M", [1, 6, 40, 200])
+def test_back_to_back_without_waiting(M):
+    """The layer kernels begin while the kernel before them still runs and wait for it before they touch memory: a chain
+    that feeds itself in place, with torch's own kernels and a group launch between, gives the same bits queued in one go
+    as with a synchronisation after every call."""
+    import torch
+    D, FF = 640, 1728
+    w_gu, w_down = (torch.from_numpy(tb.synth_packed_weights(*s)).cuda() for s in ((D, 2 * FF, 1), (FF, D, 2)))
+    gain = torch.rand(D, device="cuda") + 0.5
+    group_a = torch.zeros(1, D, dtype=torch.int8, device="cuda")
+    group_c = torch.zeros(1, 2 * FF, dtype=torch.int32, device="cuda")
+    group = tb.ProjectionGroup([(group_a, w_gu, group_c)])
+
+    def run(sync):
+        done = torch.cuda.synchronize if sync else (lambda: None)
+        g = torch.Generator(device="cuda").manual_seed(M)
+        stream = torch.randn(M, D, generator=g, device="cuda").to(torch.bfloat16)
+        x = torch.zeros_like(stream)
+        q, s = torch.empty(M, D, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+        q2, s2 = torch.empty(M, FF, dtype=torch.int8, device="cuda"), torch.empty(M, device="cuda")
+        gu = torch.empty(M, 2 * FF, dtype=torch.bfloat16, device="cuda")
+        seen = []
+        for step in range(60):
+            tb.rmsnorm_quantize(x, gain, residual=stream, out=q, row_scale=s, residual_out=stream); done()
+            tb.matmul_fused(q, w_gu, s, 0.05, out=gu); done()
+            if step % 3 == 1:
+                group_a.copy_(q[:1]); done()
+                group.run(); done()
+                seen.append(group_c.clone()); done()
+            tb.glu_quantize(gu[:, :FF], gu[:, FF:], activation="silu", eps=1e-5, out=q2, row_scale=s2); done()
+            tb.matmul_fused(q2, w_down, s2, 0.03, residual=x, out=x); done()
+            if step % 4 == 2:
+                x.mul_(0.5); done()
+        torch.cuda.synchronize()
+        return [stream, x, q, q2] + seen
+
+    want, got = run(True), run(False)
+    assert torch.isfinite(want[0]).all() and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_capture_across_streams():
+    """A layer call whose predecessors in a captured graph lie on two streams, and one that two streams follow."""
+    import torch
+    _, _, _, _, a, w, rs, cs = operands(40, 1024, 640, 3)
+    x = torch.randn(40, 1024, device="cuda").to(torch.bfloat16)
+    r = torch.randn(40, 1024, device="cuda").to(torch.bfloat16)
+    side = torch.cuda.Stream()
+
+    def work(fork):
+        main = torch.cuda.current_stream()
+        y = x * 1
+        if fork:
+            side.wait_stream(main)
+        with torch.cuda.stream(side if fork else main):
+            z = r + 1
+            q0, s0 = tb.rmsnorm_quantize(z)
+        if fork:
+            main.wait_stream(side)
+        q, s, h = tb.rmsnorm_quantize(y, residual=z)
+        if fork:
+            side.wait_stream(main)
+        with torch.cuda.stream(side if fork else main):
+            o1 = tb.matmul_fused(q, w, s, cs)
+        o2 = tb.matmul_fused(q0, w, s0, cs, activation="relu2")
+        if fork:
+            main.wait_stream(side)
+        return q, s, h, o1, o2
+
+    want = work(False)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = work(True)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
