@@ -93,6 +93,9 @@ struct StoreInt32 {
 };
 
 // k32: the output and the residual are float32; else 16 bits wide, bfloat16 or float16 by out_dtype.
+// All its operands may have been written by the kernel before, which this one may have overlapped up to dependent_wait():
+// they are read with ordinary loads, never through the read-only path (whose loads a compiler may move and whose data has
+// to hold for the kernel's whole life).
 template <bool k32>
 struct FusedEpilogue {
     static constexpr bool kFused = true;
@@ -107,12 +110,12 @@ struct FusedEpilogue {
     int bias_dtype, act, out_dtype;
     int vec4;                      // four columns from a multiple of four can be moved as one access (out and residual)
 
-    __device__ __forceinline__ float column_scale(int col) const { return col_scale ? __ldg(col_scale + col) : w_scale; }
+    __device__ __forceinline__ float column_scale(int col) const { return col_scale ? col_scale[col] : w_scale; }
     __device__ __forceinline__ float column_bias(int col) const {
         if (!bias) return 0.0f;
-        if (bias_dtype == kDtypeF32) return __ldg(static_cast<const float*>(bias) + col);
-        if (bias_dtype == kDtypeBf16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(bias) + col));
-        return __half2float(__ldg(static_cast<const __half*>(bias) + col));
+        if (bias_dtype == kDtypeF32) return static_cast<const float*>(bias)[col];
+        if (bias_dtype == kDtypeBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[col]);
+        return __half2float(static_cast<const __half*>(bias)[col]);
     }
     // Before the activation.  Without a bias 0 is added, which only turns -0 into +0.
     __device__ __forceinline__ float linear(int32_t c, float rs, float cs, float b) const {
@@ -137,7 +140,7 @@ struct FusedEpilogue {
         }
     }
     __device__ __forceinline__ void store(int row, int col, int32_t c) const {
-        float v[1] = {linear(c, __ldg(row_scale + row), column_scale(col), column_bias(col))};
+        float v[1] = {linear(c, row_scale[row], column_scale(col), column_bias(col))};
         activate(act, v);
         finish(row, col, v[0]);
     }
@@ -198,7 +201,7 @@ struct FusedEpilogue {
     }
     __device__ __forceinline__ void store4(int row, int col, const int32_t (&c)[4]) const {
         const Raw raw = load_residual4(row, col);
-        const float rs = __ldg(row_scale + row);
+        const float rs = row_scale[row];
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = linear(c[i], rs, column_scale(col + i), column_bias(col + i));

@@ -275,7 +275,7 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
                 rs[u] = 0.0f;
                 if (row[u] < M && col < N) {
                     raw[u] = epi.load_residual4(row[u], col);
-                    rs[u] = __ldg(epi.row_scale + row[u]);
+                    rs[u] = epi.row_scale[row[u]];
                 }
             }
 #pragma unroll

@@ -557,7 +557,7 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 const int t = static_cast<int>((warp & 3) * 32 + lane), c = w.w_t * kTc3TileW + rank * 128 + static_cast<int>(colp);
                 if (t < 32 * kSteps) {
                     const int row = a_t * TA + 32 * (eg + kTc3EpiGroups * (t >> 5)) + (t & 31);
-                    sts_u32(rs_sa + 4 * t, row < M ? __float_as_uint(__ldg(epi.row_scale + row)) : 0u);
+                    sts_u32(rs_sa + 4 * t, row < M ? __float_as_uint(epi.row_scale[row]) : 0u);
                 }
                 if (c < N) { col_s = epi.column_scale(c); col_b = epi.column_bias(c); }
                 const int row = a_t * TA + static_cast<int>((warp - kTc3FirstEpilogueWarp) * 32 + lane);

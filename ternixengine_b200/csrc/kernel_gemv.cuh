@@ -119,14 +119,22 @@ ternary_gemv_kernel(const __grid_constant__ CUtensorMap tmap_w, const int8_t* __
                 const int r = i / (a_len >> 2), kk = (i % (a_len >> 2)) * 4;
                 int v = 0;
                 if (row0 + r < M && k_begin + kk < K)   // K % 4 == 0 here, so a word is all-in or all-out
-                    v = *reinterpret_cast<const int*>(A + static_cast<size_t>(row0 + r) * K + k_begin + kk);
+                {
+                    const int8_t* src = A + static_cast<size_t>(row0 + r) * K + k_begin + kk;
+                    if constexpr (Epi::kFused) v = static_cast<int>(ld_ordered_u32(src));
+                    else v = *reinterpret_cast<const int*>(src);
+                }
                 *reinterpret_cast<int*>(a_s + r * krange + kk) = v;
             }
         } else {
             for (int i = tid; i < MR * a_len; i += kGemvConsumerWarps * 32) {
                 const int r = i / a_len, kk = i % a_len;
                 int8_t v = 0;
-                if (row0 + r < M && k_begin + kk < K) v = A[static_cast<size_t>(row0 + r) * K + k_begin + kk];
+                if (row0 + r < M && k_begin + kk < K) {
+                    const int8_t* src = A + static_cast<size_t>(row0 + r) * K + k_begin + kk;
+                    if constexpr (Epi::kFused) v = ld_ordered_s8(src);
+                    else v = *src;
+                }
                 a_s[r * krange + kk] = v;
             }
         }

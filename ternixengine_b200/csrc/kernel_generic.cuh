@@ -115,7 +115,7 @@ static_assert(kGenFlush % kGenK == 0, "flushes fall between slabs");
 
 template <typename Epi>
 __global__ void __launch_bounds__(kGenThreads)
-ternary_generic_fused_kernel(const int8_t* __restrict__ A, const uint8_t* __restrict__ W, int M, int K, int N, const Epi epi) {
+ternary_generic_fused_kernel(const int8_t* A, const uint8_t* W, int M, int K, int N, const Epi epi) {        // no __restrict__: see epilogue.cuh
     __shared__ __align__(16) uint32_t sA[kGenRows][kGenK / 4];
     __shared__ uint32_t sW[kGenK / 4][kGenBytes];
 

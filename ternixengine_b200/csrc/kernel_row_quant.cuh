@@ -101,18 +101,18 @@ __device__ __forceinline__ void row_pack(RowRaw<T, V>& x, const float (&v)[V]) {
 template <typename T, int V>
 __device__ __forceinline__ void row_load_weight(const void* w, int w_is_f32, int k, float (&v)[V]) {
     if constexpr (V == 1) {
-        v[0] = w_is_f32 ? __ldg(static_cast<const float*>(w) + k) : to_float<T>(static_cast<const T*>(w)[k]);
+        v[0] = w_is_f32 ? static_cast<const float*>(w)[k] : to_float<T>(static_cast<const T*>(w)[k]);
     } else {
         if (w_is_f32) {
             const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + k);
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) {
-                const float4 f = __ldg(p + i);
+                const float4 f = p[i];
                 v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
             }
         } else {
             RowRaw<T, V> x;
-            x.u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w) + k));
+            x.u = *reinterpret_cast<const uint4*>(static_cast<const T*>(w) + k);
             row_unpack<T, V>(x, v);
         }
     }

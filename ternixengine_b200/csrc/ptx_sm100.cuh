@@ -212,6 +212,18 @@ __device__ __forceinline__ void dependent_wait() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Loads that stay behind dependent_wait() and off the read-only path, whatever the pointer's qualifiers promise.
+__device__ __forceinline__ uint32_t ld_ordered_u32(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ int8_t ld_ordered_s8(const int8_t* p) {
+    int v;
+    asm volatile("ld.global.s8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return static_cast<int8_t>(v);
+}
+
 // ---------------------------------------------------------------- clusters / distributed smem
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;

@@ -1359,13 +1359,13 @@ int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int
 
 // Which kernel takes a fused product.  One row: the GEMV, unless the weights are so many (24 MB) that the clustered
 // mma.sync kernel's streaming pays (8192 x 28672: 23.8 against 18.1 us; 4096 x 11008: 7.7 against 9.0).  Two rows of few
-// weights likewise (2560 x 2560: 4.9 against 6.1 us).  Up to 8 rows mma.sync, which reads the weights once at one row group;
+// weights likewise (2560 x 2560: 4.9 against 6.1 us); more rows where only A is in the way of TMA, up to 2 MB of weights.  Up to 8 rows mma.sync, which reads the weights once at one row group;
 // from 9 rows (two row groups' worth of instructions) the prefill forms, as soon as one wave of clusters covers N
 // (16 x 6912 x 2560: 9.0 against 12.9 us; 16 x 8192 x 28672, two waves: 31.8 against 27.5), and from 17 rows always.
 int select_fused(const void* dA, const void* dW, int M, int K, int N) {
     const double w_bytes = static_cast<double>(K) * N / 4;
     const bool mma = decode_mma_ok(dA, dW, M, K, N);
-    if (gemv_ok(dW, M, K, N) && (M == 1 || (M == 2 && w_bytes <= 6e6) || !mma) && !(mma && w_bytes >= 24e6))
+    if (gemv_ok(dW, M, K, N) && (M == 1 || (M == 2 && w_bytes <= 6e6) || (!mma && w_bytes <= 2e6)) && !(mma && w_bytes >= 24e6))
         return TERNIX_B200_KERNEL_GEMV;
     if (mma && (M <= 8 || (M <= 16 && (N + tb200::kTc3TileW - 1) / tb200::kTc3TileW > sm_count() / 2)))
         return TERNIX_B200_KERNEL_DECODE_MMA;
@@ -1431,7 +1431,7 @@ int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, 
         // 6 (1 x 1000 x 4004: 6.1 against 26 us) to 10 us (129 x 1029 x 2052: 10 against 31; 1024 x 100 x 1028: 11.4 against 7.6).
         const double slabs = (K + tb200::kGenK - 1) / tb200::kGenK;
         const double tiles = static_cast<double>((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes) * ((M + tb200::kGenRows - 1) / tb200::kGenRows);
-        if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 && slabs * std::max(1.0, tiles / sm_count()) > 4)
+        if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 && N <= 0x7fffff00 && slabs * std::max(1.0, tiles / sm_count()) > 4)
             return launch_fused_aligned_copy(dA, dW, M, K, N, epi, d_status, st);
     }
     if (kernel != TERNIX_B200_KERNEL_GENERIC) return launch_fused_tma(kernel, dA, dW, M, K, N, Pitches{}, epi, d_status, st);
