@@ -199,6 +199,53 @@ struct FusedEpilogue {
             else { o[0] = lo & 0xffffu; o[1] = lo >> 16; o[2] = hi & 0xffffu; o[3] = hi >> 16; }
         }
     }
+    // R rows of four activated values (fp32 bits) each, all inside the output, vec4 only: the choices are made once.
+    template <int R>
+    __device__ __forceinline__ void finish_rows(int row, int col, const uint4 (&y)[R], const Raw* raw) const {
+        constexpr int kBytes = k32 ? 4 : 2;
+        char* o = static_cast<char*>(out) + (static_cast<size_t>(row) * ldo + col) * kBytes;
+        const size_t step = static_cast<size_t>(ldo) * kBytes;
+        float v[R][4];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            v[j][0] = __uint_as_float(y[j].x); v[j][1] = __uint_as_float(y[j].y);
+            v[j][2] = __uint_as_float(y[j].z); v[j][3] = __uint_as_float(y[j].w);
+        }
+        if constexpr (k32) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (residual) {
+                    v[j][0] = __fadd_rn(v[j][0], __uint_as_float(raw[j].x)); v[j][1] = __fadd_rn(v[j][1], __uint_as_float(raw[j].y));
+                    v[j][2] = __fadd_rn(v[j][2], __uint_as_float(raw[j].z)); v[j][3] = __fadd_rn(v[j][3], __uint_as_float(raw[j].w));
+                }
+                *reinterpret_cast<float4*>(o + j * step) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+            }
+        } else if (out_dtype == kDtypeBf16) {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (residual) {
+                    v[j][0] = __fadd_rn(v[j][0], __uint_as_float(raw[j].x << 16)); v[j][1] = __fadd_rn(v[j][1], __uint_as_float(raw[j].x & 0xffff0000u));
+                    v[j][2] = __fadd_rn(v[j][2], __uint_as_float(raw[j].y << 16)); v[j][3] = __fadd_rn(v[j][3], __uint_as_float(raw[j].y & 0xffff0000u));
+                }
+                uint2 b;
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(v[j][1]), "f"(v[j][0]));
+                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(v[j][3]), "f"(v[j][2]));
+                *reinterpret_cast<uint2*>(o + j * step) = b;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                if (residual) {
+                    v[j][0] = __fadd_rn(v[j][0], from_bits(raw[j].x & 0xffffu)); v[j][1] = __fadd_rn(v[j][1], from_bits(raw[j].x >> 16));
+                    v[j][2] = __fadd_rn(v[j][2], from_bits(raw[j].y & 0xffffu)); v[j][3] = __fadd_rn(v[j][3], from_bits(raw[j].y >> 16));
+                }
+                uint2 b;
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(b.x) : "f"(v[j][1]), "f"(v[j][0]));
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(b.y) : "f"(v[j][3]), "f"(v[j][2]));
+                *reinterpret_cast<uint2*>(o + j * step) = b;
+            }
+        }
+    }
     __device__ __forceinline__ void store4(int row, int col, const int32_t (&c)[4]) const {
         const Raw raw = load_residual4(row, col);
         const float rs = row_scale[row];

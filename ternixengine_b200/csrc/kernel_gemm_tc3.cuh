@@ -618,10 +618,14 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                         uint4 y[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) y[j] = lds_v4(buf + ((8 * q + h + j) * 128 + 4 * lane) * 4);
+                        if (epi.vec4 && col0 + 128 <= N && first + 8 <= M) {
+                            epi.finish_rows(first + h, col, y, raw + (kAhead == 4 ? 0 : h));
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float f[4] = {__uint_as_float(y[j].x), __uint_as_float(y[j].y), __uint_as_float(y[j].z), __uint_as_float(y[j].w)};
-                            if (col < N && first + h + j < M) epi.finish4(first + h + j, col, f, raw[(h + j) % kAhead]);
+                            for (int j = 0; j < 4; ++j) {
+                                const float f[4] = {__uint_as_float(y[j].x), __uint_as_float(y[j].y), __uint_as_float(y[j].z), __uint_as_float(y[j].w)};
+                                if (col < N && first + h + j < M) epi.finish4(first + h + j, col, f, raw[(h + j) % kAhead]);
+                            }
                         }
                         if (kAhead == 4 && h == 0) {
 #pragma unroll
