@@ -199,8 +199,17 @@ struct FusedEpilogue {
             else { o[0] = lo & 0xffffu; o[1] = lo >> 16; o[2] = hi & 0xffffu; o[3] = hi >> 16; }
         }
     }
-    // R rows of four activated values (fp32 bits) each, all inside the output, vec4 only: the choices are made once.
+    // The residual of R rows, all inside the output, vec4 only.
     template <int R>
+    __device__ __forceinline__ void load_residual_rows(int row, int col, Raw* raw) const {
+        constexpr int kBytes = k32 ? 4 : 2;
+        const char* p = static_cast<const char*>(residual) + (static_cast<size_t>(row) * ldr + col) * kBytes;
+        const size_t step = static_cast<size_t>(ldr) * kBytes;
+#pragma unroll
+        for (int j = 0; j < R; ++j) raw[j] = *reinterpret_cast<const Raw*>(p + j * step);
+    }
+    // R rows of four activated values (fp32 bits) each, all inside the output, vec4 only: the choices are made once.
+    template <int R, bool kRes>
     __device__ __forceinline__ void finish_rows(int row, int col, const uint4 (&y)[R], const Raw* raw) const {
         constexpr int kBytes = k32 ? 4 : 2;
         char* o = static_cast<char*>(out) + (static_cast<size_t>(row) * ldo + col) * kBytes;
@@ -214,7 +223,7 @@ struct FusedEpilogue {
         if constexpr (k32) {
 #pragma unroll
             for (int j = 0; j < R; ++j) {
-                if (residual) {
+                if constexpr (kRes) {
                     v[j][0] = __fadd_rn(v[j][0], __uint_as_float(raw[j].x)); v[j][1] = __fadd_rn(v[j][1], __uint_as_float(raw[j].y));
                     v[j][2] = __fadd_rn(v[j][2], __uint_as_float(raw[j].z)); v[j][3] = __fadd_rn(v[j][3], __uint_as_float(raw[j].w));
                 }
@@ -223,7 +232,7 @@ struct FusedEpilogue {
         } else if (out_dtype == kDtypeBf16) {
 #pragma unroll
             for (int j = 0; j < R; ++j) {
-                if (residual) {
+                if constexpr (kRes) {
                     v[j][0] = __fadd_rn(v[j][0], __uint_as_float(raw[j].x << 16)); v[j][1] = __fadd_rn(v[j][1], __uint_as_float(raw[j].x & 0xffff0000u));
                     v[j][2] = __fadd_rn(v[j][2], __uint_as_float(raw[j].y << 16)); v[j][3] = __fadd_rn(v[j][3], __uint_as_float(raw[j].y & 0xffff0000u));
                 }
@@ -235,7 +244,7 @@ struct FusedEpilogue {
         } else {
 #pragma unroll
             for (int j = 0; j < R; ++j) {
-                if (residual) {
+                if constexpr (kRes) {
                     v[j][0] = __fadd_rn(v[j][0], from_bits(raw[j].x & 0xffffu)); v[j][1] = __fadd_rn(v[j][1], from_bits(raw[j].x >> 16));
                     v[j][2] = __fadd_rn(v[j][2], from_bits(raw[j].y & 0xffffu)); v[j][3] = __fadd_rn(v[j][3], from_bits(raw[j].y >> 16));
                 }

@@ -274,10 +274,10 @@ __device__ __forceinline__ void sts_u16(uint32_t saddr, uint16_t v) {
 // tensor memory (a stage passes in half the time, the latency of a TMA load stays what it is).
 // Epi = FusedEpilogue: an epilogue warp takes its accumulator registers through scales, bias and activation in place and
 // writes them to the staging buffer as fp32; the group's four warps read that back row by row, four columns to a lane,
-// for coalesced loads of the residual and stores of the output (256 bytes of bfloat16 per row and warp) at any pitch,
-// without a TMA view.  Eight warps per CTA hold the accumulator, so what they do is bound by latency, not by issue slots:
+// for coalesced loads of the residual (kRes: there is one) and stores of the output (256 bytes of bfloat16 per row and
+// warp) at any pitch, without a TMA view.  Eight warps per CTA hold the accumulator, so what they do is bound by latency, not by issue slots:
 // done row by row on four values at a time (the first form) an epilogue of 256 x 256 took 12 us and K = 2560 waited for it.
-template <bool kGrouped, bool kBf16 = false, int TA = kTc3TileA, typename Epi = StoreInt32>
+template <bool kGrouped, bool kBf16 = false, int TA = kTc3TileA, typename Epi = StoreInt32, bool kRes = false>
 __global__ void __launch_bounds__(kTc3Threads, 1)
 ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                         const __grid_constant__ Tc3Stores stores, int32_t* __restrict__ C, int M, int K, int N,
@@ -605,21 +605,31 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                     // Row by row from here: a warp has eight rows, a lane four columns.  The residual is requested before the
                     // barrier, so that its latency is met once per step (four rows at a time in float32).
                     const int col = col0 + 4 * lane, first = row0 + 8 * static_cast<int>(q);
+                    const bool whole = epi.vec4 && col0 + 128 <= N && first + 8 <= M;
                     constexpr int kAhead = sizeof(typename Epi::Raw) == 8 ? 8 : 4;
                     typename Epi::Raw raw[kAhead];
+                    auto load_raw = [&](int row) {
+                        if constexpr (kRes) {
+                            if (sizeof(typename Epi::Raw) == 8 && whole) {        // (in float32 the unpredicated loads cost spills)
+                                epi.template load_residual_rows<kAhead>(row, col, raw);
+                            } else {
 #pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        raw[j] = typename Epi::Raw{};
-                        if (col < N && first + j < M) raw[j] = epi.load_residual4(first + j, col);
-                    }
+                                for (int j = 0; j < kAhead; ++j) {
+                                    raw[j] = typename Epi::Raw{};
+                                    if (col < N && row + j < M) raw[j] = epi.load_residual4(row + j, col);
+                                }
+                            }
+                        }
+                    };
+                    load_raw(first);
                     asm volatile("bar.sync %0, 128;" ::"r"(2 + eg) : "memory");
 #pragma unroll
                     for (int h = 0; h < 8; h += 4) {
                         uint4 y[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) y[j] = lds_v4(buf + ((8 * q + h + j) * 128 + 4 * lane) * 4);
-                        if (epi.vec4 && col0 + 128 <= N && first + 8 <= M) {
-                            epi.finish_rows(first + h, col, y, raw + (kAhead == 4 ? 0 : h));
+                        if (whole) {
+                            epi.template finish_rows<4, kRes>(first + h, col, y, raw + h % kAhead);
                         } else {
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
@@ -627,11 +637,7 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                                 if (col < N && first + h + j < M) epi.finish4(first + h + j, col, f, raw[(h + j) % kAhead]);
                             }
                         }
-                        if (kAhead == 4 && h == 0) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (col < N && first + 4 + j < M) raw[j] = epi.load_residual4(first + 4 + j, col);
-                        }
+                        if (kAhead == 4 && h == 0) load_raw(first + 4);
                     }
                     __syncwarp();
                     continue;

@@ -167,7 +167,7 @@ struct Options {
     int skinny_lo = 33, skinny_hi = 64; // rows of a single product served by the tensor-memory decode kernel (0,0 = never)
     int skinny_group_lo = 17, skinny_group_hi = 128;   // the same for members of a problem group (one launch serves many products there)
     int skinny_split = 1;              // 0: never share a block between CTAs; 1: only when blocks outnumber SMs; 2: whenever it evens the load
-    int split_rows = 0, split_cut = 0; // fused product: tile rows (64|128|256) and pairs per tile (1|2|4) of the cut prefill form; 0 = by shape
+    int split_rows = 0, split_cut = 0; // fused product: tile rows (64|128|256; 1: the persistent form) and pairs per tile (1|2|4) of the cut prefill form; 0 = by shape
     int layer_pdl = 1;                 // layer kernels as programmatic dependents of the kernel before them
     int host_slab = -1;                // slab extent of the pipelined host-pointer call; 0 = off, -1 = plan
     bool host_slab_rows = false;
@@ -646,11 +646,11 @@ int make_tc3_store_map(CUtensorMap* out, int32_t* dC, int M, int N, long long ld
     return make_tmap_2d_u32(out, dC, static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(ldc) * 4, 128, 32);
 }
 
-template <int TA, typename Epi>
+template <int TA, typename Epi, bool kRes = false>
 int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const tb200::Tc3Stores& stores, int32_t* dC0,
                            int M, int K, int N, long long ldc, int32_t* d_status, const Epi& epi, cudaStream_t st) {
     constexpr size_t smem = tb200::tc3_smem_bytes<TA>() + (Epi::kFused ? tb200::kTc3FusedSmem : 0);
-    if (const int arc = ensure_smem_attr<tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>>(smem)) return arc;
+    if (const int arc = ensure_smem_attr<tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi, kRes>>(smem)) return arc;
     const long tiles = static_cast<long>((M + TA - 1) / TA) * ((N + tb200::kTc3TileW - 1) / tb200::kTc3TileW);
     const long max_pairs = sm_count() / 2;
     const int pairs = static_cast<int>(tiles < max_pairs ? tiles : max_pairs);
@@ -670,10 +670,10 @@ int launch_gemm_tc3_maps_t(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w,
     const tb200::Tc2Tile* no_tiles = nullptr;
     const int* no_first = nullptr;
     if constexpr (Epi::kFused)
-        return launch_layer(tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>, cfg.gridDim, tb200::kTc3Threads, smem, 2, st, tmap_a,
+        return launch_layer(tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi, kRes>, cfg.gridDim, tb200::kTc3Threads, smem, 2, st, tmap_a,
                             tmap_w, stores, dC0, M, K, N, ldc, no_probs, no_tiles, no_first, d_status, static_cast<const float*>(nullptr),
                             1.0f, epi);
-    else TB_CUDA(cudaLaunchKernelEx(&cfg, tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi>, tmap_a, tmap_w, stores, dC0, M, K, N, ldc,
+    else TB_CUDA(cudaLaunchKernelEx(&cfg, tb200::ternary_gemm_tc3_kernel<false, false, TA, Epi, kRes>, tmap_a, tmap_w, stores, dC0, M, K, N, ldc,
                                no_probs, no_tiles, no_first, d_status, static_cast<const float*>(nullptr), 1.0f, epi));
     return TERNIX_B200_OK;
 }
@@ -1301,17 +1301,18 @@ struct SplitPlan {
 // Tile rows and cut with the smallest estimate, in microseconds as measured on B200 for 17 to 1500 rows, K 640 to 8192 and
 // N 640 to 28672: a cluster takes a fixed time (launch, first loads, the way out) and one per k-block of its pairs; clusters
 // beyond what the device holds at once come in waves.  The persistent form pays its way in and out once and afterwards the
-// longer of a tile's MMAs and a tile's epilogue.  E.g. 256 x 6912 x 2560: 13.5 us as 128 rows, cut 2; 28.7 us persistent;
-// 1024 x 2560 x 6912: 34.8 us as 256 rows, uncut; 24 us persistent.
+// longer of a tile's MMAs and a tile's epilogue.  E.g. 300 x 6912 x 2560: 12.1 us as 128 rows, cut 2, 23.2 us persistent;
+// 1024 x 2560 x 6912: 32.5 us as 256 rows, uncut, 21.1 us persistent.
 template <typename Epi>
 SplitPlan plan_split(int M, int K, int N) {
     const Options& o = options();
     const int blocks = (K + tb200::kTc3BK - 1) / tb200::kTc3BK;
+    if (o.split_rows == 1) return {0, 1};
     if (o.split_rows == 64 || o.split_rows == 128 || o.split_rows == 256)
         return {o.split_rows, o.split_cut >= 4 && blocks >= 4 ? 4 : o.split_cut >= 2 && blocks >= 2 ? 2 : 1};
     const long w_tiles = (N + tb200::kTc3TileW - 1) / tb200::kTc3TileW;
     const long pairs = std::max(1, sm_count() / 2), tc_waves = ((M + 255L) / 256 * w_tiles + pairs - 1) / pairs;
-    double best = 9.6 + 0.58 * blocks + static_cast<double>(tc_waves - 1) * std::max(0.58 * blocks, 7.3);
+    double best = 7.6 + 0.57 * blocks + static_cast<double>(tc_waves - 1) * std::max(0.57 * blocks, 7.0);
     SplitPlan plan{0, 1};
     for (const int rows : {64, 128, 256}) {
         const long tiles = (M + rows - 1L) / rows * w_tiles;
@@ -1319,8 +1320,8 @@ SplitPlan plan_split(int M, int K, int N) {
             if (cut > blocks) continue;
             const int held = rows == 64 ? split_clusters<64, Epi>(cut) : rows == 128 ? split_clusters<128, Epi>(cut) : split_clusters<256, Epi>(cut);
             if (held <= 0) continue;
-            const double fixed = rows == 64 ? 6.9 : rows == 128 ? (cut == 1 ? 9.0 : 8.3) : (cut == 1 ? 12.6 : 10.6);
-            const double per_block = rows == 64 ? 0.30 : rows == 128 ? 0.31 : 0.55;
+            const double fixed = rows == 64 ? 5.3 : rows == 128 ? (cut == 1 ? 7.2 : 6.5) : (cut == 1 ? 9.9 : 8.2);
+            const double per_block = rows == 64 ? 0.29 : rows == 128 ? 0.30 : 0.55;
             const double t = static_cast<double>((tiles + held - 1) / held) * (fixed + per_block * ((blocks + cut - 1) / cut));
             if (t < best) { best = t; plan = {rows, cut}; }
         }
@@ -1352,20 +1353,23 @@ int launch_fused_tma(int kernel, const int8_t* dA, const uint8_t* dW, int M, int
             CUtensorMap tmap_a, tmap_w;
             if (const int rc = make_tc3_act_map(&tmap_a, dA, M, K, 256, pt.a)) return rc;
             if (const int rc = make_tc3_weight_map(&tmap_w, dW, K, N, pt.w)) return rc;
-            return launch_gemm_tc3_maps_t<256>(tmap_a, tmap_w, tb200::Tc3Stores{}, nullptr, M, K, N, N, d_status, epi, st);
+            return epi.residual
+                       ? launch_gemm_tc3_maps_t<256, Epi, true>(tmap_a, tmap_w, tb200::Tc3Stores{}, nullptr, M, K, N, N, d_status, epi, st)
+                       : launch_gemm_tc3_maps_t<256, Epi>(tmap_a, tmap_w, tb200::Tc3Stores{}, nullptr, M, K, N, N, d_status, epi, st);
         }
     }
 }
 
 // Which kernel takes a fused product.  One row: the GEMV, unless the weights are so many (24 MB) that the clustered
-// mma.sync kernel's streaming pays (8192 x 28672: 23.8 against 18.1 us; 4096 x 11008: 7.7 against 9.0).  Two rows of few
-// weights likewise (2560 x 2560: 4.9 against 6.1 us); more rows where only A is in the way of TMA, up to 2 MB of weights.  Up to 8 rows mma.sync, which reads the weights once at one row group;
-// from 9 rows (two row groups' worth of instructions) the prefill forms, as soon as one wave of clusters covers N
-// (16 x 6912 x 2560: 9.0 against 12.9 us; 16 x 8192 x 28672, two waves: 31.8 against 27.5), and from 17 rows always.
+// mma.sync kernel's streaming pays (8192 x 28672: 22.8 against 17.7 us; 4096 x 11008: 6.6 against 8.0).  Two rows of few
+// columns likewise (2560 x 2560: 4.2 against 5.5 us; 2560 x 6912: 6.3 against 5.7); more rows where only A is in the way of
+// TMA, up to 2 MB of weights.  Up to 8 rows mma.sync, which reads the weights once at one row group; from 9 rows (twice the
+// instructions) the prefill forms, as soon as one wave of clusters covers N (16 x 6912 x 2560: 7.8 against 12.5 us;
+// 16 x 8192 x 28672, two waves: 29.9 against 28.5), and from 17 rows always.
 int select_fused(const void* dA, const void* dW, int M, int K, int N) {
     const double w_bytes = static_cast<double>(K) * N / 4;
     const bool mma = decode_mma_ok(dA, dW, M, K, N);
-    if (gemv_ok(dW, M, K, N) && (M == 1 || (M == 2 && w_bytes <= 6e6) || (!mma && w_bytes <= 2e6)) && !(mma && w_bytes >= 24e6))
+    if (gemv_ok(dW, M, K, N) && (M == 1 || (M == 2 && N <= 4096 && w_bytes <= 6e6) || (!mma && w_bytes <= 2e6)) && !(mma && w_bytes >= 24e6))
         return TERNIX_B200_KERNEL_GEMV;
     if (mma && (M <= 8 || (M <= 16 && (N + tb200::kTc3TileW - 1) / tb200::kTc3TileW > sm_count() / 2)))
         return TERNIX_B200_KERNEL_DECODE_MMA;

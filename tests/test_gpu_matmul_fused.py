@@ -114,6 +114,39 @@ def test_kernels_give_the_same_bits(shape, dtype, act):
             assert (wide == 9).all(), (kernel, pad)
 
 
+FORMS = ["1,0"] + [f"{rows},{cut}" for rows in (64, 128, 256) for cut in (1, 2, 4)]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("shape", [(1, 2560, 64), (70, 144, 320), (129, 1040, 832), (300, 4112, 256), (700, 272, 1984), (257, 2560, 1344)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_prefill_forms(shape, dtype, form, option):
+    """The persistent form and every tile size and cut of the other, forced: whole and ragged tiles in both directions, fewer
+    k-blocks than pairs asked for, more clusters than the GPU holds, any pitch; the oracle's bits, nothing written outside."""
+    import torch
+    M, K, N = shape
+    t = getattr(torch, dtype)
+    a, wp, rs, cs, ta, tw, trs, tcs = operands(M, K, N, M + N)
+    c = oracle_lib.matmul(a, wp)
+    bias = torch.randn(N, device="cuda")
+    res = torch.randn(M, N, device="cuda").to(t)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    option("fused_split", form)
+    for pad in (0, 8, 3):
+        for act, b, r in (("none", None, None), ("relu2", bias, res), ("relu", None, res), ("silu", bias, None)):
+            wide = torch.full((M + 2, N + pad), 5.0, dtype=t, device="cuda")
+            y = wide[1:M + 1, pad // 2:pad // 2 + N]
+            if r is not None:
+                y.copy_(r)                                       # in place, at the output's pitch
+            tb.matmul_fused(ta, tw, trs, tcs, bias=b, activation=act, residual=y if r is not None else None, out=y, kernel="gemm_tc",
+                            status=status)
+            check(y, c, rs, cs[None, :], None if b is None else b.cpu().numpy(), act, None if r is None else r.float().cpu().numpy())
+            y.fill_(5.0)
+            assert (wide == 5).all()
+    assert tb.last_launched_kernel() == ("ternary_gemm_tc3_kernel" if form == "1,0" else "ternary_gemm_split_kernel")
+    assert int(status.item()) == 0
+
+
 def test_residual_in_place():
     import torch
     for (M, K, N) in [(1, 2560, 2560), (20, 2560, 640), (50, 1024, 640), (300, 1040, 832), (7, 129, 132), (200, 3001, 1028)]:
