@@ -204,22 +204,26 @@ template <typename T, int VPT, int V>
 __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int have, float (&t)[VPT][V], uint2 (*slots)[32], int turn) {
     const int w_is_f32 = p.w_dtype == kDtypeF32;
     float top_f = 0.0f, sum = 0.0f;
+    if (p.eps >= 0.0f) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        const int k = (threadIdx.x + j * blockDim.x) * V;
-        if (p.eps >= 0.0f) {
+        for (int j = 0; j < VPT; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum = fmaf(t[j][i], t[j][i], sum);
-        }
-        if (p.w && j < have) {
+    }
+    if (p.w) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            if (j >= have) continue;
             float w[V];
-            row_load_weight<T, V>(p.w, w_is_f32, k, w);
+            row_load_weight<T, V>(p.w, w_is_f32, (threadIdx.x + j * blockDim.x) * V, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], w[i]);
         }
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) top_f = max_nan(top_f, fabsf(t[j][i]));
-    }
     uint32_t top = __float_as_uint(top_f);
     row_reduce(top, sum, slots, turn);
     const RowScale r = row_scale_of(top, sum, p);
