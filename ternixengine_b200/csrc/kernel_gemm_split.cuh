@@ -1,7 +1,7 @@
 // Few output tiles, fused epilogue: the paired-CTA product of kernel_gemm_tc3.cuh with K cut between the pairs of a cluster.
 //
 // What bounds a product of some dozens to a few hundred rows is neither memory nor the tensor cores of the whole GPU but
-// the few SMs that have a tile: 256 x 6912 x 2560 is ten 256 x 256 tiles, ten pairs out of 74, and each works through 27
+// the few SMs that have a tile: 256 x 6912 x 2560, say, is ten 256 x 256 tiles, ten pairs out of 74, and each works through 27
 // k-blocks of 0.5 us.  So a tile belongs to a cluster of `cut` pairs (2, 4 or 8 CTAs); pair p multiplies the p-th share of
 // the k-blocks with the machinery of the prefill kernel (weights decoded into tensor memory as the A operand, activations
 // from TMA as the B operand, cta_group::2), moves its partial sums to its own shared memory, row-major, over the
@@ -9,6 +9,12 @@
 // the pairs through distributed shared memory and takes the sums through the epilogue: four columns to a lane, a row to a
 // warp, coalesced residual loads and stores.  Integer sums: any order gives the same bits.  One tile per cluster, no
 // persistence: there is nothing after it to overlap with.
+//
+// Measured on B200 (launches in a graph, weights in L2): a cluster takes 5 to 8 us from its launch to its last store and
+// 0.3 us per k-block of its pairs up to 128 rows (two issuers; with one 0.5), 0.55 us at 256 rows.  256 x 6912 x 2560 onto a
+// residual 12 us (persistent 23 us; floor by the measured tensor rate 2.7 us); 32 x 4096 x 11008 with bias and SiLU 11 us
+// (mma.sync 15 us); 64 x 2560 x 2560 6.8 us.  What the 0.3 us hang on is not identified: four issuers, a deeper operand
+// ring (6 slots) and more expander warps leave it there; the packed-weight box has 32-byte rows, 256 requests a k-block.
 // TA: activation rows of a tile (64, 128 or 256), the pair instruction's N.
 #pragma once
 #include <cuda.h>
