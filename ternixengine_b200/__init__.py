@@ -417,9 +417,9 @@ def matmul_dequant(a, w_packed, row_scale, w_scale: float, out=None, status=None
 
 
 # --------------------------------------------------------------------------- a quantised layer around the product
-# These three run in a decode loop between kernels of a few microseconds, so their host side is kept short: one pass over
-# each operand's type, device, shape and strides, the stream's address without a Stream object, no device guard where the
-# operands' device is current already.
+# These three run in a decode loop between kernels of a few microseconds, so their host side is kept short.  Where the caller
+# gives every output and the operands' device is current, _layer_calls (csrc/layer_calls.cpp) checks and launches; it answers
+# None for anything else, malformed operands included, and the code below allocates, guards or says what is wrong.
 ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5}
 
 
@@ -435,6 +435,14 @@ class _Runtime:
         self.empty, self.Tensor, self.guard = torch.empty, torch.Tensor, torch.cuda.device
         self.scale_types = (torch.float32,)
         self.current_device, self.raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        try:
+            from . import _layer_calls as calls
+        except ImportError as e:
+            raise ImportError("_layer_calls is missing: build it with `make -C ternixengine_b200/csrc`") from e
+        entries = (lib.ternix_b200_rmsnorm_quantize, lib.ternix_b200_glu_quantize, lib.ternix_b200_matmul_fused)
+        calls.setup((torch.float32, torch.bfloat16, torch.float16, torch.int8, torch.uint8), torch.Tensor, self.current_device,
+                    self.raw_stream, *(ctypes.cast(f, ctypes.c_void_p).value for f in entries))
+        self.norm, self.glu, self.product = calls.rmsnorm_quantize, calls.glu_quantize, calls.matmul_fused
 
 
 _runtime = None
@@ -489,7 +497,9 @@ def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None,
     type or float32, or None.  Returns (codes, row_scale), and h as a third where a residual is given; residual_out may be
     `residual` or `x` itself.  codes x row_scale stands for y: codes = rint(h * weight * 127 / max|h * weight|).  A row of
     zeros has codes 0 and scale 1, a row with an infinity or NaN has codes 0 and scale NaN."""
-    rt = _rt()
+    rt = _runtime or _rt()
+    if out is not None and row_scale is not None and rt.norm(x, weight, residual, eps, out, row_scale, residual_out) == 0:
+        return (out, row_scale) if residual is None else (out, row_scale, residual_out)
     dtype = x.dtype
     code, dev, shape = rt.codes.get(dtype), x.get_device(), x.shape
     if code is None or dev < 0 or len(shape) != 2:
@@ -528,12 +538,14 @@ def glu_quantize(gate, up, activation: str = "silu", weight=None, eps=None, out=
     of one product's output.  activation: "none", "relu", "relu2", "silu", "gelu" or "gelu_tanh".  weight: (K,) of the same
     type or float32, only with eps.  Returns (codes, row_scale); rows of zeros and rows with an infinity or NaN as in
     rmsnorm_quantize()."""
-    rt = _rt()
+    rt = _runtime or _rt()
+    act = ACTIVATIONS.get(activation)
+    if out is not None and row_scale is not None and rt.glu(gate, up, act, weight, eps, out, row_scale) == 0:
+        return out, row_scale
     dtype = gate.dtype
     code, dev, shape = rt.codes.get(dtype), gate.get_device(), gate.shape
     if code is None or dev < 0 or len(shape) != 2:
         raise ValueError("glu_quantize takes CUDA (M, K) bfloat16, float16 or float32 tensors")
-    act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
     if weight is not None and eps is None:
@@ -565,8 +577,12 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
     w_scale: a number, or an (N,) float32 tensor.  bias: (N,) float32, bfloat16 or float16.  activation: "none", "relu",
     "relu2", "silu", "gelu" or "gelu_tanh".  residual: (M, N) of the output's type, unit column stride, any row pitch; may be
     `out` itself.  out: (M, N) bfloat16, float16 or float32, unit column stride, any row pitch; without it a new tensor of
-    out_dtype (the residual's type, else bfloat16)."""
-    rt = _rt()
+    out_dtype (the residual's type, else bfloat16).  status: an int32 on the same device, raised when a wait ran out."""
+    rt = _runtime or _rt()
+    act, kern = ACTIVATIONS.get(activation), KERNELS.get(kernel)
+    if out is not None and status is None and out_dtype is None and \
+            rt.product(a, w_packed, row_scale, w_scale, bias, act, residual, out, kern) == 0:
+        return out
     dev, sa, sw = a.get_device(), a.shape, w_packed.shape
     if dev < 0 or w_packed.get_device() != dev:
         raise ValueError("matmul_fused() takes CUDA tensors on one device")
@@ -578,7 +594,6 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
     if sw[0] != K:
         raise ValueError("inner dimensions do not match")
     N = sw[1] * 4
-    act, kern = ACTIVATIONS.get(activation), KERNELS.get(kernel)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
     if kern is None:
@@ -602,6 +617,8 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
         pb, b_dtype = _vector(bias, "bias", dev, rt.codes, N), rt.codes[bias.dtype]
     if residual is not None:
         pr, ldr = residual.data_ptr(), _rows(residual, "residual", dev, dtype, (M, N))
+    if status is not None and (status.dtype != rt.torch.int32 or status.get_device() != dev or status.numel() < 1):
+        raise ValueError(f"status must be an int32 tensor on cuda:{dev}")
     ep = _Epilogue(_vector(row_scale, "row_scale", dev, rt.scale_types, M), pc, ws, act, pb, b_dtype, code, pr, ldr)
     args = (a.data_ptr(), w_packed.data_ptr(), ep, out.data_ptr(), ldy, M, K, N, kern,
             status.data_ptr() if status is not None else None, rt.raw_stream(dev))

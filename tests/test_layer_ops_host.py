@@ -94,3 +94,25 @@ def test_restatement():
     assert abs(oracle.activate64(np.array([1.0]), "silu")[0] - 0.7310585786300049) < 1e-15
     assert abs(oracle.activate64(np.array([1.0]), "gelu")[0] - 0.8413447460685429) < 1e-15
     assert abs(oracle.activate64(np.array([1.0]), "gelu_tanh")[0] - 0.8411919906082768) < 1e-12
+
+
+def test_the_short_way_leaves_the_rest():
+    """The compiled way from Python to the C ABI answers None, with no error left behind, for whatever it does not take."""
+    import torch
+    rt = tb._rt()
+    x, q, s = torch.zeros(2, 64), torch.zeros(2, 64, dtype=torch.int8), torch.zeros(2)
+    w = torch.zeros(64, 16, dtype=torch.uint8)
+
+    class Odd:
+        dtype, shape = torch.float32, (2, 64)
+
+        def get_device(self):
+            raise RuntimeError("no device")
+
+    for call, args in [(rt.norm, ()), (rt.norm, (1,) * 7), (rt.norm, (None,) * 7), (rt.norm, (x, None, None, 1e-5, q, s, None)),
+                       (rt.norm, (x, None, None, 1, q, s, None)), (rt.norm, (Odd(), None, None, 1e-5, q, s, None)),
+                       (rt.norm, (x, None, x, 1e-5, q, s, None)), (rt.glu, ("x",) * 7), (rt.glu, (x, x, None, None, None, q, s)),
+                       (rt.glu, (x, x, 3, s, None, q, s)), (rt.glu, (Odd(), x, 3, None, None, q, s)), (rt.glu, (x, x, 1 << 70, None, None, q, s)),
+                       (rt.product, ()), (rt.product, (q, w, s, 1.0, None, 0, None, x, 0)), (rt.product, (q, w, s, 1.0, None, None, None, x, 0)),
+                       (rt.product, (Odd(), w, s, 1.0, None, 0, None, x, 0)), (rt.product, (q, w, s, "1", None, 0, None, x, None))]:
+        assert call(*args) is None
