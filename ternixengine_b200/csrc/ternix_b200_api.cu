@@ -251,9 +251,15 @@ int host_call_pool(cudaMemPool_t* out) {
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = dev;
         cudaMemPool_t p = nullptr;
-        TB_CUDA(cudaMemPoolCreate(&p, &props));
         unsigned long long keep = kPoolKeepBytes;
-        TB_CUDA(cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep));
+        // The first call may come while this or another thread captures: making a pool is no part of a capture, but the
+        // default capture mode would refuse it and void the capture.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        TB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        cudaError_t e = cudaMemPoolCreate(&p, &props);
+        if (e == cudaSuccess) e = cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        TB_CUDA(e);
         g_pools[dev] = p;
     }
     *out = g_pools[dev];

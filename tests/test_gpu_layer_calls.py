@@ -1,5 +1,8 @@
 """The layer operators' calls as a program makes them: the short way (every output given) against the long one, malformed
-operands with every output given, the same tensor twice and two host threads."""
+operands with every output given, the same tensor twice, two host threads, and a process whose first call is captured."""
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -7,6 +10,7 @@ import pytest
 import ternixengine_b200 as tb
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def padded(M, K, dtype, seed, pad=8):
@@ -168,3 +172,33 @@ def test_two_host_threads():
     for t in threads:
         t.join()
     assert not bad
+
+
+FIRST_CALL_CAPTURED = """
+import torch, ternixengine_b200 as tb
+M, K, N = {sizes}
+x = torch.randn(M, K, device="cuda").bfloat16()
+w = torch.from_numpy(tb.synth_packed_weights(K, N, 1)).cuda()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    q, s = tb.rmsnorm_quantize(x)
+    y = tb.matmul_fused(q, w, s, 0.05)
+    q2, s2 = tb.glu_quantize(y, y, activation="relu2")
+for _ in range(2):
+    x.copy_(torch.randn(M, K, device="cuda"))
+    g.replay()
+    torch.cuda.synchronize()
+    q_, s_ = tb.rmsnorm_quantize(x)
+    y_ = tb.matmul_fused(q_, w, s_, 0.05)
+    for p, r in zip((q, s, y, q2, s2), (q_, s_, y_, *tb.glu_quantize(y_, y_, activation="relu2"))):
+        assert torch.equal(p, r)
+print("replayed")
+"""
+
+
+@pytest.mark.parametrize("sizes", [(1, 2560, 640), (6, 2560, 640), (40, 2560, 640), (300, 1040, 832), (33, 1029, 1028), (3, 65, 68)])
+def test_first_call_of_a_process_is_captured(sizes):
+    """Everything that the library sets up on first use (attributes, occupancy, its pool) may happen under capture."""
+    env = dict(os.environ, PYTHONPATH=ROOT)
+    p = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED.format(sizes=sizes)], capture_output=True, text=True, timeout=300, env=env)
+    assert p.returncode == 0 and "replayed" in p.stdout, p.stderr[-2000:]
