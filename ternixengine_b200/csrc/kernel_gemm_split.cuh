@@ -2,7 +2,7 @@
 //
 // What bounds a product of some dozens to a few hundred rows is neither memory nor the tensor cores of the whole GPU but
 // the few SMs that have a tile: 256 x 6912 x 2560, say, is ten 256 x 256 tiles, ten pairs out of 74, and each works through 27
-// k-blocks of 0.5 us.  So a tile belongs to a cluster of `cut` pairs (2, 4 or 8 CTAs); pair p multiplies the p-th share of
+// k-blocks of 0.5 us.  So a tile belongs to a cluster of `cut` pairs (2, 4, 6 or 8 CTAs); pair p multiplies the p-th share of
 // the k-blocks with the machinery of the prefill kernel (weights decoded into tensor memory as the A operand, activations
 // from TMA as the B operand, cta_group::2), moves its partial sums to its own shared memory, row-major, over the
 // activation ring, which is idle by then, and after a cluster barrier every CTA adds up its share of the tile's rows over
@@ -12,8 +12,8 @@
 //
 // Measured on B200 (launches in a graph, weights in L2): a cluster takes 5 to 8 us from its launch to its last store and
 // 0.3 us per k-block of its pairs up to 128 rows (two issuers; with one 0.5), 0.55 us at 256 rows.  256 x 6912 x 2560 onto a
-// residual 12 us (persistent 23 us; floor by the measured tensor rate 2.7 us); 32 x 4096 x 11008 with bias and SiLU 11 us
-// (mma.sync 15 us); 64 x 2560 x 2560 6.8 us.  What the 0.3 us hang on is not identified: four issuers, a deeper operand
+// residual 11.3 us, cut 3 (cut 2 12.1; persistent 23 us; floor by the measured tensor rate 2.7 us); 32 x 4096 x 11008 with bias and SiLU 11 us
+// (mma.sync 15 us); 64 x 2560 x 2560 6.5 us.  What the 0.3 us hang on is not identified: four issuers, a deeper operand
 // ring (6 slots) and more expander warps leave it there; the packed-weight box has 32-byte rows, 256 requests a k-block.
 // TA: activation rows of a tile (64, 128 or 256), the pair instruction's N.
 #pragma once
@@ -224,9 +224,9 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
         if (!met) cluster_wait();
         // ================================================================ partial sums: tensor memory -> shared memory
         // The tile's residual comes into L2 meanwhile: the rows this CTA will finish, one per thread.
-        const int share = TA / cut, first = row0 + static_cast<int>(pair) * share;
+        const int share = (TA + cut - 1) / cut, first = row0 + static_cast<int>(pair) * share;
         const int mine = static_cast<int>(threadIdx.x) - kSpFirstExpandWarp * 32;
-        if (epi.residual && mine < share && first + mine < M && col0 < N) epi.prefetch_residual(first + mine, col0, min(128, N - col0));
+        if (epi.residual && mine < share && first + mine < min(M, row0 + TA) && col0 < N) epi.prefetch_residual(first + mine, col0, min(128, N - col0));
         __syncwarp();
         const uint32_t colp = q * 32 + 4 * (lane & 7) + (lane >> 3);       // the column numbering above
         const uint32_t part = smem_u32(sAct);
@@ -257,9 +257,9 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
     __syncwarp();
     cluster_sync_all();                // every pair's partial tile is in place
 
-    // ---- rows pair x TA / cut ... of the tile, this CTA's 128 columns: sums over the pairs, epilogue
+    // ---- the pair's share of the tile's rows, this CTA's 128 columns: sums over the pairs, epilogue
     {
-        const int share = TA / cut, first = static_cast<int>(pair) * share;
+        const int per_pair = (TA + cut - 1) / cut, first = static_cast<int>(pair) * per_pair, share = min(per_pair, TA - first);
         const int col = col0 + 4 * lane;
         const uint32_t part = smem_u32(sAct) + 16 * lane;
         float cs[4], b[4];

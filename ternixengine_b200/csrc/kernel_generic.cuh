@@ -205,6 +205,7 @@ align_rows_kernel(const __grid_constant__ AlignJob a, const __grid_constant__ Al
     const int per_row = job.pitch / 16, width = job.width;
     const uintptr_t lo = reinterpret_cast<uintptr_t>(job.src), hi = lo + static_cast<uintptr_t>(job.rows) * width;
     const long long total = job.rows * per_row, block = first ? blockIdx.x : blockIdx.x - a.blocks;
+    dependent_wait();
     for (long long i = block * 256 + threadIdx.x; i < total; i += job.blocks * 256LL) {
         const long long r = i / per_row;
         const int x = static_cast<int>(i - r * per_row) * 16;
@@ -217,7 +218,7 @@ align_rows_kernel(const __grid_constant__ AlignJob a, const __grid_constant__ Al
             w[j] = 0;
             if (x + 4 * j - shift / 8 >= width) continue;
             if (p >= lo && p + 4 <= hi) {
-                w[j] = __ldg(reinterpret_cast<const uint32_t*>(p));
+                w[j] = *reinterpret_cast<const uint32_t*>(p);
             } else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)

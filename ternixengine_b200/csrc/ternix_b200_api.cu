@@ -167,7 +167,7 @@ struct Options {
     int skinny_lo = 33, skinny_hi = 64; // rows of a single product served by the tensor-memory decode kernel (0,0 = never)
     int skinny_group_lo = 17, skinny_group_hi = 128;   // the same for members of a problem group (one launch serves many products there)
     int skinny_split = 1;              // 0: never share a block between CTAs; 1: only when blocks outnumber SMs; 2: whenever it evens the load
-    int split_rows = 0, split_cut = 0; // fused product: tile rows (64|128|256; 1: the persistent form) and pairs per tile (1|2|4) of the cut prefill form; 0 = by shape
+    int split_rows = 0, split_cut = 0; // fused product: tile rows (64|128|256; 1: the persistent form) and pairs per tile (1-4) of the cut prefill form; 0 = by shape
     int layer_pdl = 1;                 // layer kernels as programmatic dependents of the kernel before them
     int host_slab = -1;                // slab extent of the pipelined host-pointer call; 0 = off, -1 = plan
     bool host_slab_rows = false;
@@ -1277,8 +1277,8 @@ int launch_gemm_split_t(const int8_t* dA, const uint8_t* dW, int M, int K, int N
 // Clusters of the cut form that the device holds at once (asked once per device and form).
 template <int TA, typename Epi>
 int split_clusters(int cut) {
-    static std::atomic<int> cache[kMaxDevices][3] = {};
-    std::atomic<int>& slot = cache[current_device()][cut == 4 ? 2 : cut - 1];
+    static std::atomic<int> cache[kMaxDevices][tb200::kSpMaxCut] = {};
+    std::atomic<int>& slot = cache[current_device()][cut - 1];
     int n = slot.load(std::memory_order_relaxed);
     if (n > 0) return n;
     constexpr auto kern = tb200::ternary_gemm_split_kernel<TA, Epi>;
@@ -1307,7 +1307,7 @@ struct SplitPlan {
 // Tile rows and cut with the smallest estimate, in microseconds as measured on B200 for 17 to 1500 rows, K 640 to 8192 and
 // N 640 to 28672: a cluster takes a fixed time (launch, first loads, the way out) and one per k-block of its pairs; clusters
 // beyond what the device holds at once come in waves.  The persistent form pays its way in and out once and afterwards the
-// longer of a tile's MMAs and a tile's epilogue.  E.g. 300 x 6912 x 2560: 12.1 us as 128 rows, cut 2, 23.2 us persistent;
+// longer of a tile's MMAs and a tile's epilogue.  E.g. 256 x 6912 x 2560: 11.3 us as 128 rows, cut 3, 12.1 us cut 2, 23.2 us persistent;
 // 1024 x 2560 x 6912: 32.5 us as 256 rows, uncut, 21.1 us persistent.
 template <typename Epi>
 SplitPlan plan_split(int M, int K, int N) {
@@ -1315,20 +1315,22 @@ SplitPlan plan_split(int M, int K, int N) {
     const int blocks = (K + tb200::kTc3BK - 1) / tb200::kTc3BK;
     if (o.split_rows == 1) return {0, 1};
     if (o.split_rows == 64 || o.split_rows == 128 || o.split_rows == 256)
-        return {o.split_rows, o.split_cut >= 4 && blocks >= 4 ? 4 : o.split_cut >= 2 && blocks >= 2 ? 2 : 1};
+        return {o.split_rows, std::max(1, std::min({o.split_cut, blocks, tb200::kSpMaxCut}))};
     const long w_tiles = (N + tb200::kTc3TileW - 1) / tb200::kTc3TileW;
     const long pairs = std::max(1, sm_count() / 2), tc_waves = ((M + 255L) / 256 * w_tiles + pairs - 1) / pairs;
     double best = 7.6 + 0.57 * blocks + static_cast<double>(tc_waves - 1) * std::max(0.57 * blocks, 7.0);
     SplitPlan plan{0, 1};
     for (const int rows : {64, 128, 256}) {
         const long tiles = (M + rows - 1L) / rows * w_tiles;
-        for (const int cut : {1, 2, 4}) {
+        for (int cut = 1; cut <= tb200::kSpMaxCut; ++cut) {
             if (cut > blocks) continue;
             const int held = rows == 64 ? split_clusters<64, Epi>(cut) : rows == 128 ? split_clusters<128, Epi>(cut) : split_clusters<256, Epi>(cut);
             if (held <= 0) continue;
-            const double fixed = rows == 64 ? 5.3 : rows == 128 ? (cut == 1 ? 7.2 : 6.5) : (cut == 1 ? 9.9 : 8.2);
-            const double per_block = rows == 64 ? 0.29 : rows == 128 ? 0.30 : 0.55;
-            const double t = static_cast<double>((tiles + held - 1) / held) * (fixed + per_block * ((blocks + cut - 1) / cut));
+            // uncut, a pair writes and finishes the whole tile; with the cut the sum over the pairs grows
+            static constexpr double kFixed[3][tb200::kSpMaxCut] = {{5.3, 5.3, 5.45, 5.9}, {7.2, 6.5, 6.6, 6.9}, {9.9, 8.2, 8.3, 8.6}};
+            static constexpr double kPerBlock[3] = {0.29, 0.30, 0.55};
+            const int form = rows == 64 ? 0 : rows == 128 ? 1 : 2;
+            const double t = static_cast<double>((tiles + held - 1) / held) * (kFixed[form][cut - 1] + kPerBlock[form] * ((blocks + cut - 1) / cut));
             if (t < best) { best = t; plan = {rows, cut}; }
         }
     }
@@ -1417,9 +1419,8 @@ int launch_fused_aligned_copy(const int8_t* dA, const uint8_t* dW, int M, int K,
         w = dst;
         pt.w = w_pitch;
     }
-    tb200::align_rows_kernel<<<static_cast<unsigned>(ja.blocks + jw.blocks), 256, 0, st>>>(ja, jw);
-    const cudaError_t e = cudaGetLastError();
-    const int rc = e != cudaSuccess ? cuda_fail(e) : launch_fused_tma(kernel, a, w, M, K, N, pt, epi, d_status, st);
+    int rc = launch_layer(tb200::align_rows_kernel, dim3(static_cast<unsigned>(ja.blocks + jw.blocks)), 256, 0, 1, st, ja, jw);
+    if (rc == TERNIX_B200_OK) rc = launch_fused_tma(kernel, a, w, M, K, N, pt, epi, d_status, st);
     cudaFreeAsync(tmp, st);
     return rc;
 }
@@ -1438,7 +1439,7 @@ int launch_fused(int kernel, const int8_t* dA, const uint8_t* dW, int M, int K, 
     if (kernel == TERNIX_B200_KERNEL_AUTO) {
         kernel = select_fused(dA, dW, M, K, N);
         // The generic kernel takes 1.5 us per 64 k-rows and round of tiles; an aligned copy and the kernel behind it from
-        // 6 (1 x 1000 x 4004: 6.1 against 26 us) to 10 us (129 x 1029 x 2052: 10 against 31; 1024 x 100 x 1028: 11.4 against 7.6).
+        // 6 (1 x 1000 x 4004: 6.1 against 26 us) to 10 us (129 x 1029 x 2052: 9.7 against 31; 1024 x 100 x 1028: 11.4 against 7.6).
         const double slabs = (K + tb200::kGenK - 1) / tb200::kGenK;
         const double tiles = static_cast<double>((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes) * ((M + tb200::kGenRows - 1) / tb200::kGenRows);
         if (kernel == TERNIX_B200_KERNEL_GENERIC && K <= kMaxScaledK - 16 && N <= 0x7fffff00 && slabs * std::max(1.0, tiles / sm_count()) > 4)

@@ -114,7 +114,7 @@ def test_kernels_give_the_same_bits(shape, dtype, act):
             assert (wide == 9).all(), (kernel, pad)
 
 
-FORMS = ["1,0"] + [f"{rows},{cut}" for rows in (64, 128, 256) for cut in (1, 2, 4)]
+FORMS = ["1,0"] + [f"{rows},{cut}" for rows in (64, 128, 256) for cut in (1, 2, 3, 4)]
 
 
 @pytest.mark.parametrize("form", FORMS)
