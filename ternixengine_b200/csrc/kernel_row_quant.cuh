@@ -17,7 +17,7 @@
 // start or end off a 16-byte boundary).
 //
 // Bound by memory: each input once, each output once.  Measured on B200 (copy rate 6.55 TB/s): gate 4096 x 28672 bfloat16 with
-// squared ReLU 92 us = 6.4 TB/s; with SiLU 115 us (two MUFU instructions an element, and an SM has room for one row, so its
+// squared ReLU 91 us = 6.4 TB/s; with SiLU 112 us (two MUFU instructions an element, and an SM has room for one row, so its
 // phases do not overlap); norm with residual 4096 x 8192 bfloat16 42 us = 5.6 TB/s, float32 70 us = 6.2 TB/s; 4096 x 2560
 // bfloat16 15.8 us.  One row: 1.9 us (2560), 2.7 us (6912 with the norm), the launch and two trips through the reduction.
 #pragma once
@@ -322,13 +322,14 @@ row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
             if constexpr (kIn == 2) sts_v4(mine + (j * kIn + 1) * step, make_uint4(0, 0, 0, 0));
         }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     int turn = 0;
     for (int row = blockIdx.x; row < p.M; row += gridDim.x, turn ^= 1) {
         float t[VPT][V];
         RowRaw<T, V> x[VPT], y[VPT];
         const int next = row + static_cast<int>(gridDim.x);
         const char *nx = row_x(next), *ny = row_y(next);
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         // Each vector's slots are requested again as soon as they have been read (a thread's shared-memory accesses are
         // performed in order, and nobody else touches its slots), before any arithmetic on this row.
 #pragma unroll
@@ -337,6 +338,7 @@ row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
             y[j].u = kIn == 2 ? lds_v4(mine + (j * kIn + 1) * step) : make_uint4(0, 0, 0, 0);
             if (next < p.M) fetch(nx, ny, j);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
         row_values<T, MODE, VPT, V>(p, row, have, x, y, t);
         row_finish<T, VPT, V>(p, row, have, t, slots, turn);
     }

@@ -1223,18 +1223,24 @@ int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
     auto threads_for = [&](int items, int vpt) { return std::max(32, ((items + vpt - 1) / vpt + 31) / 32 * 32); };
     if (vec) {
         const int items = p.K / V;
-        // Rows of more than 8 KB an operand, enough of them to come in rounds: persistent CTAs with the next row under way
-        // (4096 x 8192 bfloat16 with residual 42 us against 49, 4096 x 28672 gate 88 against 119; below that size an SM holds
-        // many rows at once and nothing is gained: 4096 x 2560 16.7 us either way).  float32 with a residual moves so many
-        // bytes a row that it runs at the copy rate without (4096 x 8192: 68 us against 80).
-        constexpr bool kStream = !(sizeof(T) == 4 && MODE == tb200::kRowNormResidual);
-        if constexpr (kStream) {
-            if (items > 512 && p.M >= 2 * sm_count()) {
-                if (MODE != tb200::kRowGate && items <= 1024) return launch_row_quant_stream_t<T, MODE, 2>(p, threads_for(items, 2), st);
-                const int threads = threads_for(items, 4);
-                if (items <= 4096 && static_cast<size_t>(MODE == tb200::kRowNorm ? 64 : 128) * threads <= kRowStreamSmem)
-                    return launch_row_quant_stream_t<T, MODE, 4>(p, threads, st);
-            }
+        // Many long rows: persistent CTAs with the next row under way.  Up to 1024 vectors a row the narrow form (three CTAs of
+        // 512 threads an SM), from 20 rows per SM the one of 4 vectors a thread, which then pays from 320 vectors on (bfloat16,
+        // us without | with: norm 4096 x 8192 35.7 | 24.4, 8192 x 4096 33.1 | 24.4, 2048 x 6912 18.5 | 13.0 narrow, 4096 x 2560
+        // 12.3 | 11.3; gate 4096 x 6912 38.0 | 27.9, 4096 x 28672 137 | 111; 4096 x 1280 7.5 | 8.2).  With a residual a row is
+        // three streams of bytes and an SM is full sooner: the narrow form up to 1024 vectors (4096 x 8192 46.1 | 42.3, float32
+        // 4096 x 4096 35.6 | 37.5, so not there), nothing up to 2048 (4096 x 14336 66.2 | 76.6), beyond, where an SM holds one
+        // row, the wide form again (4096 x 20480 112 | 100, float32 2560 x 10000 72 | 64).
+        const bool many = p.M >= 20 * sm_count(), some = p.M >= 2 * sm_count();
+        if constexpr (MODE == tb200::kRowNormResidual) {
+            if (sizeof(T) == 2 && items <= 1024 && ((some && items > 512) || (many && items > 320)))
+                return launch_row_quant_stream_t<T, MODE, 2>(p, threads_for(items, 2), st);
+        } else if (items <= 1024 && some && !many && items > 512) {
+            return launch_row_quant_stream_t<T, MODE, 2>(p, threads_for(items, 2), st);
+        }
+        if (MODE == tb200::kRowNormResidual ? some && items > 2048 : (many && items > 320) || (some && items > 1024)) {
+            const int threads = threads_for(items, 4);
+            if (items <= 4096 && static_cast<size_t>(MODE == tb200::kRowNorm ? 64 : 128) * threads <= kRowStreamSmem)
+                return launch_row_quant_stream_t<T, MODE, 4>(p, threads, st);
         }
         if (items <= 512) return launch_row_quant_t<T, MODE, 1, true>(p, threads_for(items, 1), st);
         if (items <= 1024) return launch_row_quant_t<T, MODE, 2, true>(p, threads_for(items, 2), st);

@@ -175,6 +175,52 @@ def test_residual_in_place_and_pitches():
             assert torch.equal(wide, keep_w) and torch.equal(res, keep_r)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [297, 2961])
+@pytest.mark.parametrize("vectors", [320, 321, 513, 1024, 1025, 2048, 2049, 4096])
+def test_many_rows(dtype, M, vectors):
+    """What is chosen by the number of rows: the rows as above in calls of fewer rows, where nothing of it runs.  Codes and h
+    are the same bits; scales within twice the bound of a sum (another order).  Zero and poisoned rows between others, any
+    pitch of whole vectors, the residual stream in place."""
+    import torch
+    t = getattr(torch, dtype)
+    V = 4 if dtype == "float32" else 8
+    K = vectors * V
+
+    def pitched(seed, pad):
+        return make((M, K + pad), dtype, seed)[:, :K]
+
+    x, r, w = pitched(1, 2 * V), pitched(2, V), (torch.randn(K, device="cuda") * 0.3 + 1).to(t)
+    x[5:M:97] = 0
+    r[5:M:97] = 0
+    x[11:M:131, K // 3] = float("nan")
+    r[200, K - 1] = float("inf")
+    tol = 2 * oracle.row_scale_bound(K)
+
+    def same(got, pieces):
+        for i, part in enumerate(pieces):
+            rows = slice(100 * i, 100 * i + part[0].shape[0])
+            assert torch.equal(got[0][rows], part[0])
+            a, b = got[1][rows].double(), part[1].double()
+            assert torch.equal(a.isnan(), b.isnan()) and bool(((a - b).abs() <= b * tol)[~b.isnan()].all())
+            if len(got) == 3:
+                assert torch.equal(got[2][rows].nan_to_num(nan=77.0), part[2].nan_to_num(nan=77.0))
+
+    def pieces(f):
+        return [f(slice(i, min(i + 100, M))) for i in range(0, M, 100)]
+
+    same(tb.rmsnorm_quantize(x, w), pieces(lambda s: tb.rmsnorm_quantize(x[s], w)))
+    want = pieces(lambda s: tb.glu_quantize(x[s], r[s], activation="silu", weight=w, eps=1e-5))
+    same(tb.glu_quantize(x, r, activation="silu", weight=w, eps=1e-5), want)
+    want = pieces(lambda s: tb.glu_quantize(x[s], r[s], activation="relu2"))
+    same(tb.glu_quantize(x, r, activation="relu2"), want)
+    want = pieces(lambda s: tb.rmsnorm_quantize(x[s], w, residual=r[s]))
+    same(tb.rmsnorm_quantize(x, w, residual=r), want)
+    got = tb.rmsnorm_quantize(x, w, residual=r, residual_out=r)
+    assert got[2] is r
+    same(got, want)
+
+
 def test_outputs_of_the_caller_and_empty_sizes():
     import torch
     x = make((9, 640), "bfloat16", 1)
