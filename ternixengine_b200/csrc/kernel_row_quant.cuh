@@ -13,8 +13,10 @@
 // the NaN-propagating instruction and carried between lanes as bits (|NaN| > inf > any finite as integers).
 // 127 / m would overflow for m below 2^-121; such rows are scaled up by 2^100 first, which is exact.
 //
-// A row belongs to one CTA, spread over its threads as VPT vectors of 16 bytes each (or as single elements, where rows
-// start or end off a 16-byte boundary).
+// A row belongs to one CTA, spread over its threads as VPT vectors of 16 bytes each.  Where rows start or end off a 16-byte
+// boundary the vectors are laid out so that their codes are aligned (the first and the last one may be partial), and a
+// vector of an input is put together from the two aligned pieces that it lies in: odd rows, and the halves of a product's
+// output with an odd width.
 //
 // Bound by memory: each input once, each output once.  Measured on B200 (copy rate 6.55 TB/s): gate 4096 x 28672 bfloat16 with
 // squared ReLU 91 us = 6.4 TB/s; with SiLU 112 us (two MUFU instructions an element, and an SM has room for one row, so its
@@ -122,16 +124,74 @@ __device__ __forceinline__ void row_load_weight(const void* w, int w_is_f32, int
         }
     }
 }
-// A thread's part of a row, loaded as x and y, as what is normalised and quantised (h or z); h is written on the way.
+// 16 bytes at any element's address: the two aligned pieces that hold them (requested first, put together by shift16() when
+// they have arrived), or, where a piece reaches beyond [lo, hi), element by element with zeros outside; nothing outside is read.
+struct Piece16 {
+    uint4 a, b;
+    bool whole;
+};
+template <typename E, bool kAligned>
+__device__ __forceinline__ Piece16 load16(const char* at, const char* lo, const char* hi) {
+    Piece16 r;
+    const char* a = kAligned ? at : at - (reinterpret_cast<uintptr_t>(at) & 15);
+    r.whole = a >= lo && a + (kAligned ? 16 : 32) <= hi;
+    if (r.whole) {
+        r.a = *reinterpret_cast<const uint4*>(a);
+        r.b = kAligned ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(a + 16);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; i += static_cast<int>(sizeof(E))) {
+            if (at + i < lo || at + i >= hi) continue;
+            if constexpr (sizeof(E) == 4) w[i / 4] = *reinterpret_cast<const uint32_t*>(at + i);
+            else w[i / 4] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + i)) << (8 * (i & 3));
+        }
+        r.a = make_uint4(w[0], w[1], w[2], w[3]);
+        r.b = make_uint4(0, 0, 0, 0);
+    }
+    return r;
+}
+__device__ __forceinline__ uint4 shift16(const Piece16& p, const char* at) {
+    const uint32_t off = p.whole ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at)) & 15 : 0;
+    const uint32_t w[8] = {p.a.x, p.a.y, p.a.z, p.a.w, p.b.x, p.b.y, p.b.z, p.b.w};
+    uint32_t v[6], z[5];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) v[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) z[i] = off & 4 ? v[i + 1] : v[i];
+    const uint32_t bits = (off & 3) * 8;
+    return make_uint4(__funnelshift_r(z[0], z[1], bits), __funnelshift_r(z[1], z[2], bits), __funnelshift_r(z[2], z[3], bits),
+                      __funnelshift_r(z[3], z[4], bits));
+}
+// The weights of columns k .. k + V - 1 where they are not a vector of their own; zeros outside the row.
+template <typename T, int V>
+__device__ __forceinline__ void row_load_weight_shifted(const void* w, int w_is_f32, int k, int K, float (&v)[V]) {
+    const char* lo = static_cast<const char*>(w);
+    if (w_is_f32) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const char* at = lo + (static_cast<long long>(k) + i) * 4;
+            const uint4 u = shift16(load16<float, false>(at, lo, lo + static_cast<long long>(K) * 4), at);
+            v[i] = __uint_as_float(u.x); v[i + 1] = __uint_as_float(u.y); v[i + 2] = __uint_as_float(u.z); v[i + 3] = __uint_as_float(u.w);
+        }
+    } else {
+        RowRaw<T, V> x;
+        const char* at = lo + static_cast<long long>(k) * static_cast<int>(sizeof(T));
+        x.u = shift16(load16<T, false>(at, lo, lo + static_cast<long long>(K) * static_cast<int>(sizeof(T))), at);
+        row_unpack<T, V>(x, v);
+    }
+}
+// A thread's part of a row, loaded as x and y, as what is normalised and quantised (h or z); h is written on the way.  Vector
+// j starts at column (threadIdx.x + j blockDim.x) V - shift; kVec: shift is 0 and every vector whole and aligned.
 // `have`: how many of its VPT vectors lie inside the row; the others are zero and stay zero under every activation.
-template <typename T, int MODE, int VPT, int V>
-__device__ __forceinline__ void row_values(const RowQuantArgs& p, int row, int have, RowRaw<T, V> (&x)[VPT],
+template <typename T, int MODE, int VPT, int V, bool kVec>
+__device__ __forceinline__ void row_values(const RowQuantArgs& p, int row, int have, int shift, RowRaw<T, V> (&x)[VPT],
                                            const RowRaw<T, V> (&y)[VPT], float (&t)[VPT][V]) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) row_unpack<T, V>(x[j], t[j]);
     if constexpr (MODE == kRowGate) activate(p.act, reinterpret_cast<float (&)[VPT * V]>(t));       // one choice for all of them
     if constexpr (MODE != kRowNorm) {
-        T* h = MODE == kRowNormResidual ? static_cast<T*>(p.h) + static_cast<size_t>(row) * p.ldh + threadIdx.x * V : nullptr;
+        T* h = MODE == kRowNormResidual ? static_cast<T*>(p.h) + static_cast<long long>(row) * p.ldh + static_cast<int>(threadIdx.x * V) - shift : nullptr;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             float o[V];
@@ -141,7 +201,19 @@ __device__ __forceinline__ void row_values(const RowQuantArgs& p, int row, int h
                 for (int i = 0; i < V; ++i) t[j][i] = __fadd_rn(t[j][i], o[i]);
                 row_pack<T, V>(x[j], t[j]);
                 row_unpack<T, V>(x[j], t[j]);
-                if (j < have) x[j].store(h + j * blockDim.x * V);
+                if constexpr (kVec) {
+                    if (j < have) x[j].store(h + j * blockDim.x * V);
+                } else {
+                    const int k = static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift;
+                    T* at = h + j * blockDim.x * V;
+                    if (k >= 0 && k + V <= p.K && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+                        x[j].store(at);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            if (k + i >= 0 && k + i < p.K) at[i] = x[j].t[i];
+                    }
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], o[i]);
@@ -205,8 +277,8 @@ __device__ __forceinline__ void row_store_scale(const RowQuantArgs& p, int row, 
 }
 
 // One row, held in registers as t: statistics, scale, codes.  `slots` and `turn` as in row_reduce().
-template <typename T, int VPT, int V>
-__device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int have, float (&t)[VPT][V], uint2 (*slots)[32], int turn) {
+template <typename T, int VPT, int V, bool kVec>
+__device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int have, int shift, float (&t)[VPT][V], uint2 (*slots)[32], int turn) {
     const int w_is_f32 = p.w_dtype == kDtypeF32;
     float top_f = 0.0f, sum = 0.0f;
     if (p.eps >= 0.0f) {
@@ -220,7 +292,8 @@ __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int h
         for (int j = 0; j < VPT; ++j) {
             if (j >= have) continue;
             float w[V];
-            row_load_weight<T, V>(p.w, w_is_f32, (threadIdx.x + j * blockDim.x) * V, w);
+            if constexpr (kVec) row_load_weight<T, V>(p.w, w_is_f32, (threadIdx.x + j * blockDim.x) * V, w);
+            else row_load_weight_shifted<T, V>(p.w, w_is_f32, static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift, p.K, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], w[i]);
         }
@@ -233,7 +306,7 @@ __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int h
     row_reduce(top, sum, slots, turn);
     const RowScale r = row_scale_of(top, sum, p);
     if (threadIdx.x == 0) row_store_scale(p, row, top, sum, r);
-    int8_t* q = p.q + static_cast<size_t>(row) * p.K + threadIdx.x * V;
+    int8_t* q = p.q + static_cast<long long>(row) * p.K + static_cast<int>(threadIdx.x * V) - shift;
     if (r.lift != 1.0f) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
@@ -244,49 +317,81 @@ __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int h
     for (int j = 0; j < VPT; ++j) {
         if (j >= have) continue;
         int8_t* at = q + j * blockDim.x * V;
-        if constexpr (V == 1) {
-            *at = static_cast<int8_t>(row_code(t[j][0], r.inv) & r.keep);
-        } else {
-            uint32_t c[V / 4];
+        uint32_t c[V / 4];
 #pragma unroll
-            for (int i = 0; i < V / 4; ++i)
-                c[i] = pack_codes(row_code(t[j][4 * i], r.inv), row_code(t[j][4 * i + 1], r.inv),
-                                  row_code(t[j][4 * i + 2], r.inv), row_code(t[j][4 * i + 3], r.inv)) & r.keep;
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(c[0], c[1]);
-            else *reinterpret_cast<uint32_t*>(at) = c[0];
+        for (int i = 0; i < V / 4; ++i)
+            c[i] = pack_codes(row_code(t[j][4 * i], r.inv), row_code(t[j][4 * i + 1], r.inv),
+                              row_code(t[j][4 * i + 2], r.inv), row_code(t[j][4 * i + 3], r.inv)) & r.keep;
+        if constexpr (!kVec) {
+            const int k = static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift;
+            if (k < 0 || k + V > p.K) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (k + i >= 0 && k + i < p.K) at[i] = static_cast<int8_t>(c[i / 4] >> (8 * (i & 3)));
+                continue;
+            }
         }
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(c[0], c[1]);
+        else *reinterpret_cast<uint32_t*>(at) = c[0];
     }
 }
-// Vectors of a row that fall to this thread: threadIdx.x, threadIdx.x + blockDim.x, ... below K / V.
-template <int V>
-__device__ __forceinline__ int row_have(int K) {
-    const int left = K / V - static_cast<int>(threadIdx.x);
+// Of `items` vectors those that fall to this thread: threadIdx.x, threadIdx.x + blockDim.x, ...
+__device__ __forceinline__ int row_have(int items) {
+    const int left = items - static_cast<int>(threadIdx.x);
     return left <= 0 ? 0 : (left + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
 }
 
-// One row per CTA.
-template <typename T, int MODE, int VPT, bool kVec>
+// One row per CTA.  Of a row's operands and codes: all on vector boundaries; all equally far off one; anything else.
+constexpr int kRowAligned = 0, kRowSamePhase = 1, kRowAnyPhase = 2;
+template <typename T, int MODE, int VPT, int kForm>
 __global__ void __launch_bounds__(1024)
 row_quant_kernel(const __grid_constant__ RowQuantArgs p) {
-    constexpr int V = kVec ? kRowVec<T> : 1;
+    constexpr int V = kRowVec<T>;
+    constexpr bool kVec = kForm == kRowAligned, kSame = kForm == kRowSamePhase;
     __shared__ uint2 slots[2][32];
-    const int row = blockIdx.x, have = row_have<V>(p.K);
+    const int row = blockIdx.x;
+    int shift = 0;
+    if constexpr (!kVec) shift = static_cast<int>((reinterpret_cast<uintptr_t>(p.q) + static_cast<uintptr_t>(row) * p.K) & (V - 1));
+    const int have = row_have(kVec ? p.K / V : (shift + p.K + V - 1) / V);
     dependent_wait();
     float t[VPT][V];
     // all of the row's loads first: a store of h between them would hold the next ones back (h may be x or y)
     RowRaw<T, V> x[VPT], y[VPT];
-    const T* px = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx + threadIdx.x * V;
-    const T* py = MODE == kRowNorm ? nullptr : static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy + threadIdx.x * V;
+    const T* px = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx;
+    const T* py = MODE == kRowNorm ? nullptr : static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy;
+    if constexpr (kVec) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        x[j].u = y[j].u = make_uint4(0, 0, 0, 0);
-        if (j < have) {
-            x[j].load(px + j * blockDim.x * V);
-            if constexpr (MODE != kRowNorm) y[j].load(py + j * blockDim.x * V);
+        for (int j = 0; j < VPT; ++j) {
+            x[j].u = y[j].u = make_uint4(0, 0, 0, 0);
+            if (j < have) {
+                x[j].load(px + (threadIdx.x + j * blockDim.x) * V);
+                if constexpr (MODE != kRowNorm) y[j].load(py + (threadIdx.x + j * blockDim.x) * V);
+            }
+        }
+    } else {
+        const char *xl = reinterpret_cast<const char*>(px), *yl = reinterpret_cast<const char*>(py);
+        const long long bytes = static_cast<long long>(p.K) * static_cast<int>(sizeof(T));
+        auto offset = [&](int j) {
+            return (static_cast<long long>(threadIdx.x + j * blockDim.x) * V - shift) * static_cast<int>(sizeof(T));
+        };
+        Piece16 a[VPT], b[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            a[j].a = a[j].b = b[j].a = b[j].b = make_uint4(0, 0, 0, 0);
+            a[j].whole = b[j].whole = false;
+            if (j < have) {
+                a[j] = load16<T, kSame>(xl + offset(j), xl, xl + bytes);
+                if constexpr (MODE != kRowNorm) b[j] = load16<T, kSame>(yl + offset(j), yl, yl + bytes);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            x[j].u = kSame ? a[j].a : shift16(a[j], xl + offset(j));
+            y[j].u = MODE == kRowNorm ? make_uint4(0, 0, 0, 0) : kSame ? b[j].a : shift16(b[j], yl + offset(j));
         }
     }
-    row_values<T, MODE, VPT, V>(p, row, have, x, y, t);
-    row_finish<T, VPT, V>(p, row, have, t, slots, 0);
+    row_values<T, MODE, VPT, V, kVec>(p, row, have, shift, x, y, t);
+    row_finish<T, VPT, V, kVec>(p, row, have, shift, t, slots, 0);
 }
 
 // Many rows: persistent CTAs that have the next row under way while they reduce and quantise this one.  A thread copies
@@ -301,7 +406,7 @@ row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
     extern __shared__ __align__(16) uint4 row_stage[];             // [VPT][kIn][threads]
     __shared__ uint2 slots[2][32];
     const uint32_t mine = smem_u32(row_stage) + threadIdx.x * 16, step = blockDim.x * 16;
-    const int have = row_have<V>(p.K);
+    const int have = row_have(p.K / V);
     const size_t stride = static_cast<size_t>(blockDim.x) * 16;              // bytes between a thread's vectors
     auto fetch = [&](const char* x, const char* y, int j) {
         if (j >= have) return;
@@ -339,8 +444,8 @@ row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
             if (next < p.M) fetch(nx, ny, j);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        row_values<T, MODE, VPT, V>(p, row, have, x, y, t);
-        row_finish<T, VPT, V>(p, row, have, t, slots, turn);
+        row_values<T, MODE, VPT, V, true>(p, row, have, 0, x, y, t);
+        row_finish<T, VPT, V, true>(p, row, have, 0, t, slots, turn);
     }
 }
 

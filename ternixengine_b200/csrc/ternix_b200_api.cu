@@ -1191,9 +1191,9 @@ bool dtype_ok(int d) { return d == TERNIX_B200_DTYPE_F32 || d == TERNIX_B200_DTY
 int dtype_bytes(int d) { return d == TERNIX_B200_DTYPE_F32 ? 4 : 2; }
 bool activation_ok(int a) { return a >= TERNIX_B200_ACT_NONE && a <= TERNIX_B200_ACT_GELU_TANH; }
 
-template <typename T, int MODE, int VPT, bool kVec>
+template <typename T, int MODE, int VPT, int kForm>
 int launch_row_quant_t(const tb200::RowQuantArgs& p, int threads, cudaStream_t st) {
-    return launch_layer(tb200::row_quant_kernel<T, MODE, VPT, kVec>, dim3(static_cast<unsigned>(p.M)), threads, 0, 1, st, p);
+    return launch_layer(tb200::row_quant_kernel<T, MODE, VPT, kForm>, dim3(static_cast<unsigned>(p.M)), threads, 0, 1, st, p);
 }
 constexpr size_t kRowStreamSmem = 200 * 1024;
 template <typename T, int MODE, int VPT>
@@ -1242,12 +1242,26 @@ int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
             if (items <= 4096 && static_cast<size_t>(MODE == tb200::kRowNorm ? 64 : 128) * threads <= kRowStreamSmem)
                 return launch_row_quant_stream_t<T, MODE, 4>(p, threads, st);
         }
-        if (items <= 512) return launch_row_quant_t<T, MODE, 1, true>(p, threads_for(items, 1), st);
-        if (items <= 1024) return launch_row_quant_t<T, MODE, 2, true>(p, threads_for(items, 2), st);
-        if (items <= 4096) return launch_row_quant_t<T, MODE, 4, true>(p, threads_for(items, 4), st);
+        if (items <= 512) return launch_row_quant_t<T, MODE, 1, tb200::kRowAligned>(p, threads_for(items, 1), st);
+        if (items <= 1024) return launch_row_quant_t<T, MODE, 2, tb200::kRowAligned>(p, threads_for(items, 2), st);
+        if (items <= 4096) return launch_row_quant_t<T, MODE, 4, tb200::kRowAligned>(p, threads_for(items, 4), st);
     } else {
-        if (p.K <= 4096) return launch_row_quant_t<T, MODE, 4, false>(p, threads_for(p.K, 4), st);
-        if (p.K <= 16384) return launch_row_quant_t<T, MODE, 16, false>(p, threads_for(p.K, 16), st);
+        const long long items = (p.K + 2LL * V - 2) / V;          // a row's vectors wherever it starts
+        auto phase = [&](const void* q, long long ld) {            // whether a row of it is as far off a vector as the row's codes
+            return !q || ((reinterpret_cast<uintptr_t>(q) / sizeof(T) - reinterpret_cast<uintptr_t>(p.q)) % V == 0 && (p.M == 1 || (ld - p.K) % V == 0));
+        };
+        const bool same = phase(p.x, p.ldx) && phase(p.y, p.ldy) && phase(p.h, p.ldh);
+        // Two vectors a thread as long as a CTA has an SM to itself (1 x 8191 norm with residual 3.2 us, four 4.2), else four,
+        // whose CTAs are small enough for three an SM (4096 x 8191: 59.5 us, two 68.0; element by element it was 92.8).
+        auto launch = [&](auto form) {
+            constexpr int kForm = decltype(form)::value;
+            const int n = static_cast<int>(items);
+            if (n <= 512) return launch_row_quant_t<T, MODE, 1, kForm>(p, threads_for(n, 1), st);
+            if (n <= 2048 && p.M <= sm_count()) return launch_row_quant_t<T, MODE, 2, kForm>(p, threads_for(n, 2), st);
+            return launch_row_quant_t<T, MODE, 4, kForm>(p, threads_for(n, 4), st);
+        };
+        if (items <= 4096)
+            return same ? launch(std::integral_constant<int, tb200::kRowSamePhase>{}) : launch(std::integral_constant<int, tb200::kRowAnyPhase>{});
     }
     return launch_layer(tb200::row_quant_long_kernel<T, MODE>, dim3(static_cast<unsigned>(p.M)), 1024, 0, 1, st, p);
 }

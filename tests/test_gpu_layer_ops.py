@@ -221,6 +221,54 @@ def test_many_rows(dtype, M, vectors):
     same(got, want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [3, 150])
+@pytest.mark.parametrize("K", [1, 5, 9, 641, 2561, 4099, 8191, 16375, 16401, 32761])
+def test_rows_off_a_vector_boundary(dtype, M, K):
+    """Odd rows without gaps (every operand equally far off a boundary), and every operand at an offset and pitch of its own;
+    weights off a boundary in both types.  Nothing outside the rows is read into them or written."""
+    import torch
+    t = getattr(torch, dtype)
+    nan = float("nan")
+
+    def at(offset, pitch, values, fill):
+        """`values` in rows of `pitch` from element `offset` of a buffer that holds `fill` otherwise."""
+        flat = torch.full((offset + M * pitch + 16,), fill, dtype=values.dtype, device="cuda")
+        view = flat[offset:offset + M * pitch].view(M, pitch)[:, :K]
+        view.copy_(values)
+        return flat, view
+
+    x0, r0 = make((M, K), dtype, K), make((M, K), dtype, K + 1)
+    w0 = torch.randn(K, device="cuda") * 0.3 + 1
+    h0 = (x0.float() + r0.float()).to(t)
+    ms = (to_np(h0).astype(np.float64) ** 2).mean(axis=1)
+    for layout in (((0, K), (0, K), (0, K), 0, 0), ((1, K + 3), (2, K + 2), (3, K + 5), 1, 1), ((3, K), (0, K + 1), (5, K), 3, 2)):
+        (xo, xp), (ro, rp), (ho, hp), qo, wo = layout
+        for w_type in (None, torch.float32, t):
+            w = None if w_type is None else torch.cat([torch.full((wo,), nan, device="cuda"), w0]).to(w_type)[wo:]
+            (_, x), (_, r) = at(xo, xp, x0, nan), at(ro, rp, r0, nan)
+            h_flat, h = at(ho, hp, torch.full_like(x0, 5), 5)
+            q_flat = torch.full((M * K + 32,), 55, dtype=torch.int8, device="cuda")
+            q, s = q_flat[qo:qo + M * K].view(M, K), torch.empty(M, device="cuda")
+            tb.rmsnorm_quantize(x, w, residual=r, out=q, row_scale=s, residual_out=h)
+            assert torch.equal(h, h0)
+            v = to_np(h0) if w is None else (to_np(h0) * to_np(w)[None, :]).astype(np.float32)
+            check_quantized(q, s, v, ms, 1e-5, K)
+            h.fill_(5)
+            assert (h_flat == 5).all()
+            tb.rmsnorm_quantize(h0 if xo == 0 else at(xo, xp, h0, nan)[1], w, out=q, row_scale=s)
+            check_quantized(q, s, v, ms, 1e-5, K)
+            z = (np.where(to_np(x0) < 0, np.float32(0), to_np(x0)) * to_np(r0)).astype(np.float32)
+            eps = None if w is None else 1e-5
+            tb.glu_quantize(x, r, activation="relu", weight=w, eps=eps, out=q, row_scale=s)
+            check_quantized(q, s, z if w is None else (z * to_np(w)[None, :]).astype(np.float32), (z.astype(np.float64) ** 2).mean(axis=1), eps, K)
+            q.fill_(55)
+            assert (q_flat == 55).all()
+            want = tb.rmsnorm_quantize(x, w, residual=r)
+            got = tb.rmsnorm_quantize(x, w, residual=r, residual_out=x)          # in place
+            assert got[2] is x and torch.equal(x, h0) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_outputs_of_the_caller_and_empty_sizes():
     import torch
     x = make((9, 640), "bfloat16", 1)
