@@ -54,6 +54,24 @@ __device__ __forceinline__ float rcp_approx(float x) {
 __device__ __forceinline__ float logistic_times(float v, float u) {
     return v * rcp_approx(1.0f + exp2_approx(-1.44269504f * u));
 }
+// log2 of P(v) / P(-v) over v, P the normal distribution: v P(v), the exact GELU, is v / (1 + 2^(-that v)).  Odd in v and smooth, so
+// a polynomial in v^2; this one is a least-squares fit in Chebyshev points of v^2 on [0, 32], weighted by P(v) P(-v) and reweighted
+// (Lawson's method) until the error in P is level: 1.2e-8.  Beyond v^2 = 32 it stays constant, where P is within 1e-8 of 0 or 1.
+// P is then off by at most 1.2e-7 (the fit, P (1 - P) times the exponential's 2^-22 and its argument's roundings) and 2^-22 of
+// itself (sum, reciprocal, product), as little as with the library's erf, whose form took 98 us where this one takes 68 (4096 x
+// 2560 x 6912; SiLU 54) and 167 where it takes 124 (gate 4096 x 28672; SiLU 112).
+__device__ __forceinline__ float gelu_logit(float v) {
+    const float u = fminf(__fmul_rn(v, v), 32.0f);
+    float r = -1.0653262e-11f;
+    r = fmaf(r, u, 6.922505e-10f);
+    r = fmaf(r, u, -1.1965207e-08f);
+    r = fmaf(r, u, -1.775779e-07f);
+    r = fmaf(r, u, 1.01666847e-05f);
+    r = fmaf(r, u, -1.5548168e-04f);
+    r = fmaf(r, u, -1.0037289e-04f);
+    r = fmaf(r, u, 0.10483905f);
+    return fmaf(r, u, 2.3022087f);
+}
 // act(v) on N values at once: the choice is the same for the whole launch, so it is made once per N values.  A NaN stays
 // a NaN in every activation.
 template <int N>
@@ -76,7 +94,7 @@ __device__ __forceinline__ void activate(int act, float (&v)[N]) {
             break;
         case kActGelu:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
+            for (int i = 0; i < N; ++i) v[i] = v[i] * rcp_approx(1.0f + exp2_approx(-__fmul_rn(v[i], gelu_logit(v[i]))));
             break;
         case kActGeluTanh:       // 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
 #pragma unroll
