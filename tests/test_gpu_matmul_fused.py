@@ -214,6 +214,33 @@ def test_extreme_values_and_depth():
             assert torch.equal(y[keep], want[act][keep])
 
 
+@pytest.mark.parametrize("M,N", [(1, 1 << 18), (24, 1 << 16), (300, 1 << 13)])
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_over_their_range(act, M, N):
+    """Every activation from the smallest floats to the largest, through the bias of a product of zeros: the float64 function
+    within its error (what rounds to zero or to its argument included), the limits at infinity, NaN."""
+    import torch
+    rng = np.random.default_rng(N)
+    parts = [np.linspace(-30, 30, N // 2), np.geomspace(1e-38, 1e18, N // 8), -np.geomspace(1e-38, 1e18, N // 8),
+             rng.normal(size=N - N // 2 - 2 * (N // 8) - 64) * 3, np.zeros(64)]
+    v = np.concatenate(parts).astype(F)
+    v[-4:] = [np.inf, -np.inf, np.nan, F(3e38) if act != "relu2" else F(1e19)]
+    a, w = torch.zeros(M, 64, dtype=torch.int8, device="cuda"), torch.zeros(64, N // 4, dtype=torch.uint8, device="cuda")
+    y = tb.matmul_fused(a, w, torch.ones(M, device="cuda"), 1.0, bias=torch.from_numpy(v).cuda(), activation=act, out_dtype=torch.float32)
+    assert torch.equal(y[:1].expand_as(y).isnan(), y.isnan()) and torch.equal(y[:1].nan_to_num().expand_as(y), y.nan_to_num())
+    got = y[0].cpu().numpy()
+    end = [got[-4], got[-3], got[-2]]
+    assert end[0] == np.inf and np.isnan(end[2])
+    assert end[1] == (0 if act.startswith("relu") else -np.inf) if act in ("none", "relu", "relu2") else np.isnan(end[1])
+    v, got = np.delete(v, [N - 4, N - 3, N - 2]), np.delete(got, [N - 4, N - 3, N - 2]).astype(np.float64)
+    want = oracle.activate64(v, act)
+    with np.errstate(over="ignore", invalid="ignore"):
+        tol = oracle.activation_error(v, act)
+    tol = np.nan_to_num(tol, nan=0.0) + np.abs(want) * 2.0 ** -24 + np.finfo(F).smallest_normal      # flushed to zero below it
+    off = np.abs(got - want) - tol
+    assert (off <= 0).all(), (act, v[np.argmax(off)], got[np.argmax(off)], want[np.argmax(off)])
+
+
 def test_empty_sizes():
     import torch
     a = torch.empty((3, 0), dtype=torch.int8, device="cuda")
