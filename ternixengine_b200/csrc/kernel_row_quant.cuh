@@ -13,7 +13,7 @@
 // the NaN-propagating instruction and carried between lanes as bits (|NaN| > inf > any finite as integers).
 // 127 / m would overflow for m below 2^-121; such rows are scaled up by 2^100 first, which is exact.
 //
-// A row belongs to one CTA, spread over its threads as VPT vectors of 16 bytes each.  Where rows start or end off a 16-byte
+// A row belongs to one CTA (a cluster, where rows are few and long), spread over its threads as VPT vectors of 16 bytes each.  Where rows start or end off a 16-byte
 // boundary the vectors are laid out so that their codes are aligned (the first and the last one may be partial), and a
 // vector of an input is put together from the two aligned pieces that it lies in: odd rows, and the halves of a product's
 // output with an odd width.
@@ -21,7 +21,8 @@
 // Bound by memory: each input once, each output once.  Measured on B200 (copy rate 6.55 TB/s): gate 4096 x 28672 bfloat16 with
 // squared ReLU 91 us = 6.4 TB/s; with SiLU 112 us (two MUFU instructions an element, and an SM has room for one row, so its
 // phases do not overlap); norm with residual 4096 x 8192 bfloat16 42 us = 5.6 TB/s, float32 70 us = 6.2 TB/s; 4096 x 2560
-// bfloat16 15.8 us.  One row: 1.9 us (2560), 2.7 us (6912 with the norm), the launch and two trips through the reduction.
+// bfloat16 15.8 us.  One row: 1.9 us (2560), 2.2 us (6912 gate with the norm, a
+// cluster of eight), 2.4 us (28672), the launch and two trips through the reduction.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -247,6 +248,29 @@ __device__ __forceinline__ void row_reduce(uint32_t& top, float& sum, uint2 (*sl
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
 }
 
+// The same over the CTAs of a cluster, at most 64 warps in all: a warp's result goes into its slot in every CTA, and each adds
+// up the same slots in the same order.  The caller has arrived at the cluster's barrier once, so that nobody is written to
+// before it runs; behind the second round nobody touches a peer again.
+constexpr int kWideSlots = 64;
+__device__ __forceinline__ void row_reduce_cluster(uint32_t& top, float& sum, uint2* slots, uint32_t rank, uint32_t ctas) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, n = warps * static_cast<int>(ctas);
+    top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    cluster_wait();
+    if (lane < static_cast<int>(ctas))
+        asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(dsmem_map(smem_u32(&slots[rank * warps + warp]), lane)), "r"(top),
+                     "r"(__float_as_uint(sum)) : "memory");
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const uint2 a = lane < n ? slots[lane] : make_uint2(0, 0), b = lane + 32 < n ? slots[lane + 32] : make_uint2(0, 0);
+    top = __reduce_max_sync(0xffffffffu, max(a.x, b.x));
+    sum = __uint_as_float(a.y) + __uint_as_float(b.y);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+}
+
 // What the statistics of a row say about its codes: q = rint((t * lift) * inv), all zero where keep is 0.
 struct RowScale {
     float lift, inv;
@@ -276,9 +300,10 @@ __device__ __forceinline__ void row_store_scale(const RowQuantArgs& p, int row, 
     p.row_scale[row] = scale;
 }
 
-// One row, held in registers as t: statistics, scale, codes.  `slots` and `turn` as in row_reduce().
-template <typename T, int VPT, int V, bool kVec>
-__device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int have, int shift, float (&t)[VPT][V], uint2 (*slots)[32], int turn) {
+// One row (or a CTA's part of it), held in registers as t: statistics, scale, codes.  reduce(top, sum): as row_reduce().
+template <typename T, int VPT, int V, bool kVec, typename Reduce>
+__device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int have, int shift, float (&t)[VPT][V], bool store_scale,
+                                           const Reduce& reduce) {
     const int w_is_f32 = p.w_dtype == kDtypeF32;
     float top_f = 0.0f, sum = 0.0f;
     if (p.eps >= 0.0f) {
@@ -292,7 +317,7 @@ __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int h
         for (int j = 0; j < VPT; ++j) {
             if (j >= have) continue;
             float w[V];
-            if constexpr (kVec) row_load_weight<T, V>(p.w, w_is_f32, (threadIdx.x + j * blockDim.x) * V, w);
+            if constexpr (kVec) row_load_weight<T, V>(p.w, w_is_f32, static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift, w);
             else row_load_weight_shifted<T, V>(p.w, w_is_f32, static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift, p.K, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) t[j][i] = __fmul_rn(t[j][i], w[i]);
@@ -303,9 +328,9 @@ __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int h
 #pragma unroll
         for (int i = 0; i < V; ++i) top_f = max_nan(top_f, fabsf(t[j][i]));
     uint32_t top = __float_as_uint(top_f);
-    row_reduce(top, sum, slots, turn);
+    reduce(top, sum);
     const RowScale r = row_scale_of(top, sum, p);
-    if (threadIdx.x == 0) row_store_scale(p, row, top, sum, r);
+    if (threadIdx.x == 0 && store_scale) row_store_scale(p, row, top, sum, r);
     int8_t* q = p.q + static_cast<long long>(row) * p.K + static_cast<int>(threadIdx.x * V) - shift;
     if (r.lift != 1.0f) {
 #pragma unroll
@@ -391,7 +416,35 @@ row_quant_kernel(const __grid_constant__ RowQuantArgs p) {
         }
     }
     row_values<T, MODE, VPT, V, kVec>(p, row, have, shift, x, y, t);
-    row_finish<T, VPT, V, kVec>(p, row, have, shift, t, slots, 0);
+    row_finish<T, VPT, V, kVec>(p, row, have, shift, t, true, [&](uint32_t& top, float& sum) { row_reduce(top, sum, slots, 0); });
+}
+
+// A few long rows, all on vector boundaries: a row belongs to a cluster, each CTA has a part of it.
+template <typename T, int MODE, int VPT>
+__global__ void __launch_bounds__(256)
+row_quant_wide_kernel(const __grid_constant__ RowQuantArgs p) {
+    constexpr int V = kRowVec<T>;
+    __shared__ uint2 slots[kWideSlots];
+    const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
+    const int row = blockIdx.x / ctas, items = p.K / V, part = (items + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+    const int first = static_cast<int>(rank) * part, have = row_have(min(part, items - first));
+    cluster_arrive();
+    dependent_wait();
+    float t[VPT][V];
+    RowRaw<T, V> x[VPT], y[VPT];
+    const T* px = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx + (first + static_cast<int>(threadIdx.x)) * V;
+    const T* py = MODE == kRowNorm ? nullptr : static_cast<const T*>(p.y) + static_cast<size_t>(row) * p.ldy + (first + static_cast<int>(threadIdx.x)) * V;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        x[j].u = y[j].u = make_uint4(0, 0, 0, 0);
+        if (j < have) {
+            x[j].load(px + j * blockDim.x * V);
+            if constexpr (MODE != kRowNorm) y[j].load(py + j * blockDim.x * V);
+        }
+    }
+    row_values<T, MODE, VPT, V, true>(p, row, have, -first * V, x, y, t);
+    row_finish<T, VPT, V, true>(p, row, have, -first * V, t, rank == 0,
+                                [&](uint32_t& top, float& sum) { row_reduce_cluster(top, sum, slots, rank, ctas); });
 }
 
 // Many rows: persistent CTAs that have the next row under way while they reduce and quantise this one.  A thread copies
@@ -445,7 +498,7 @@ row_quant_stream_kernel(const __grid_constant__ RowQuantArgs p) {
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         row_values<T, MODE, VPT, V, true>(p, row, have, 0, x, y, t);
-        row_finish<T, VPT, V, true>(p, row, have, 0, t, slots, turn);
+        row_finish<T, VPT, V, true>(p, row, have, 0, t, true, [&](uint32_t& top, float& sum) { row_reduce(top, sum, slots, turn); });
     }
 }
 

@@ -1223,6 +1223,19 @@ int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
     auto threads_for = [&](int items, int vpt) { return std::max(32, ((items + vpt - 1) / vpt + 31) / 32 * 32); };
     if (vec) {
         const int items = p.K / V;
+        // A few long rows: a cluster to each (1 x 28672 gate 5.1 | 2.4 us, 1 x 8192 norm with residual 2.9 | 2.2, 32 x 14336 3.8 | 2.9;
+        // 1 x 4096 and 128 rows gain nothing or lose).  Eight CTAs, or four where the rows alone are work for most SMs.
+        if ((p.M <= 32 && items > 512) || (p.M <= 64 && items > 1024)) {
+            const int ctas = p.M <= 8 || items > 2048 ? 8 : 4, part = (items + ctas - 1) / ctas;
+            auto wide = [&](auto vpt) {
+                constexpr int VPT = decltype(vpt)::value;
+                return launch_layer(tb200::row_quant_wide_kernel<T, MODE, VPT>, dim3(static_cast<unsigned>(p.M * ctas)), threads_for(part, VPT), 0,
+                                    ctas, st, p);
+            };
+            if (part <= 256) return wide(std::integral_constant<int, 1>{});
+            if (part <= 512) return wide(std::integral_constant<int, 2>{});
+            if (part <= 1024) return wide(std::integral_constant<int, 4>{});
+        }
         // Many long rows: persistent CTAs with the next row under way.  Up to 1024 vectors a row the narrow form (three CTAs of
         // 512 threads an SM), from 20 rows per SM the one of 4 vectors a thread, which then pays from 320 vectors on (bfloat16,
         // us without | with: norm 4096 x 8192 35.7 | 24.4, 8192 x 4096 33.1 | 24.4, 2048 x 6912 18.5 | 13.0 narrow, 4096 x 2560

@@ -222,6 +222,37 @@ def test_many_rows(dtype, M, vectors):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 8, 9, 32, 33, 64, 65])
+@pytest.mark.parametrize("vectors", [513, 1025, 2049, 4096, 8191, 8193])
+def test_a_few_long_rows(dtype, M, vectors):
+    """Rows shared by the CTAs of a cluster (whole and partial shares, the last CTA with none), and what is next to them: too
+    many rows for it, rows too long for it.  Zero rows, poisoned rows, the stream in place, any pitch of whole vectors."""
+    import torch
+    t = getattr(torch, dtype)
+    V = 4 if dtype == "float32" else 8
+    K = vectors * V
+    x, r = make((M, K + V), dtype, M)[:, :K], make((M, K + 3 * V), dtype, M + 1)[:, :K]
+    if M > 2:
+        x[0], r[0] = 0, 0
+        x[M - 1, K - 1] = float("nan")
+    for weight in (None, (torch.randn(K, device="cuda") * 0.3 + 1).to(t), torch.randn(K, device="cuda") * 0.3 + 1):
+        w = np.ones(K, dtype=np.float32) if weight is None else to_np(weight)
+        codes, scale = tb.rmsnorm_quantize(x, weight)
+        h = to_np(x)
+        check_quantized(codes, scale, (h * w).astype(np.float32), (h.astype(np.float64) ** 2).mean(axis=1), 1e-5, K)
+        z = (np.where(h < 0, np.float32(0), h) * to_np(r)).astype(np.float32)
+        codes, scale = tb.glu_quantize(x, r, activation="relu", weight=weight, eps=None if weight is None else 1e-5)
+        check_quantized(codes, scale, (z * w).astype(np.float32), (z.astype(np.float64) ** 2).mean(axis=1), None if weight is None else 1e-5, K)
+        keep = r.clone()
+        h_t = (x.float() + r.float()).to(t)
+        codes, scale, h = tb.rmsnorm_quantize(x, weight, residual=r, residual_out=r)
+        assert h is r and torch.equal(r.nan_to_num(nan=77.0), h_t.nan_to_num(nan=77.0))
+        h = to_np(h_t)
+        check_quantized(codes, scale, (h * w).astype(np.float32), (h.astype(np.float64) ** 2).mean(axis=1), 1e-5, K)
+        r.copy_(keep)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M", [3, 150])
 @pytest.mark.parametrize("K", [1, 5, 9, 641, 2561, 4099, 8191, 16375, 16401, 32761])
 def test_rows_off_a_vector_boundary(dtype, M, K):
