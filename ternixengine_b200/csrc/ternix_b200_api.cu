@@ -417,11 +417,70 @@ int launch_gemv_t(const CUtensorMap& tmap, const int8_t* dA, int32_t* dC, int M,
     return TERNIX_B200_OK;
 }
 
+// Clusters of the one-row kernel that the device holds at once (asked once per device, form and CTAs per SM).
+template <int MR, int WORDS, typename Epi>
+int gemv_clusters(int ksplit, int krange) {
+    static std::atomic<int> cache[kMaxDevices][4][4] = {};
+    const size_t smem = tb200::gemv_smem_bytes<MR, WORDS>(krange);
+    const int per_sm = std::min(3, static_cast<int>(227 * 1024 / (smem + 1024)));
+    std::atomic<int>& slot = cache[current_device()][ksplit == 8 ? 3 : ksplit / 2][per_sm];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    constexpr auto kern = tb200::ternary_gemv_kernel<MR, WORDS, Epi>;
+    if (ensure_smem_attr<kern>(tb200::gemv_smem_bytes<MR, WORDS>(tb200::kGemvMaxASlice / MR)) != TERNIX_B200_OK) return 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(ksplit));
+    cfg.blockDim = dim3(tb200::kGemvThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ksplit);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return 0;
+    }
+    slot.store(n, std::memory_order_relaxed);
+    return n;
+}
+// The fused product's plan: the smallest estimate, in microseconds as measured.  An SM takes 2.75 us for 1024 rows of 64 bytes
+// however many of its CTAs share them (3.0 with one), and clusters beyond what the device holds at once come in waves, which is
+// what plan_gemv() does not know: 1 x 2560 x 13824 as 54 clusters of 8 takes two (9.0 us), as 54 of 4 one (6.8).
+template <int MR, typename Epi>
+GemvPlan plan_gemv_fused(int M, int K, int N) {
+    const Options& o = options();
+    if (o.gemv_words || o.gemv_split) return plan_gemv(M, K, N);
+    GemvPlan best{0, 0, 0};
+    double best_time = 1e30;
+    for (const int words : {16, 32}) {
+        const int stage_rows = 8 * (32 / words) * 4;
+        const long tiles = static_cast<long>((N + words * 16 - 1) / (words * 16)) * ((M + MR - 1) / MR);
+        for (const int ks : {1, 2, 4, 8}) {
+            int krange = (K + ks - 1) / ks;
+            krange = (krange + stage_rows - 1) / stage_rows * stage_rows;
+            if (krange * 4 > tb200::kGemvMaxASlice || (ks > 1 && static_cast<long>(krange) * (ks - 1) >= K)) continue;
+            const int held = words == 16 ? gemv_clusters<MR, 16, Epi>(ks, krange) : gemv_clusters<MR, 32, Epi>(ks, krange);
+            if (held <= 0) continue;
+            const long shared = (std::min<long>(tiles, held) * ks + sm_count() - 1) / sm_count();          // CTAs of an SM
+            const double row = (shared > 1 ? 2.75e-3 : 3.0e-3) * words / 16;
+            const double t = static_cast<double>((tiles + held - 1) / held) * (2.2 + static_cast<double>(shared) * krange * row);
+            if (t < best_time) { best_time = t; best = {words, ks, krange}; }
+        }
+    }
+    return best.words ? best : plan_gemv(M, K, N);
+}
+
 // w_pitch: bytes between the k-rows of W (N / 4 in the packed format; more in a copy made for the TMA unit).
 template <typename Epi = tb200::StoreInt32>
 int launch_gemv(const int8_t* dA, const uint8_t* dW, int32_t* dC, int M, int K, int N, long long ldc,
                 int32_t* d_status, cudaStream_t st, const Epi& epi = {}, long long w_pitch = 0) {
-    const GemvPlan p = plan_gemv(M, K, N);
+    GemvPlan p;
+    if constexpr (Epi::kFused)
+        p = M == 1 ? plan_gemv_fused<1, Epi>(M, K, N) : M == 2 ? plan_gemv_fused<2, Epi>(M, K, N) : plan_gemv_fused<4, Epi>(M, K, N);
+    else p = plan_gemv(M, K, N);
     if (p.words == 0) return TERNIX_B200_ERR_UNSUPPORTED;
     const int stage_rows = 8 * (32 / p.words) * 4;
     CUtensorMap tmap;
