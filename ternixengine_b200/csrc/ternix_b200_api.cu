@@ -419,11 +419,11 @@ int launch_gemv_t(const CUtensorMap& tmap, const int8_t* dA, int32_t* dC, int M,
 
 // Clusters of the one-row kernel that the device holds at once (asked once per device, form and CTAs per SM).
 template <int MR, int WORDS, typename Epi>
-int gemv_clusters(int ksplit, int krange) {
+int gemv_clusters(int dev, int ksplit, int krange) {
     static std::atomic<int> cache[kMaxDevices][4][4] = {};
     const size_t smem = tb200::gemv_smem_bytes<MR, WORDS>(krange);
     const int per_sm = std::min(3, static_cast<int>(227 * 1024 / (smem + 1024)));
-    std::atomic<int>& slot = cache[current_device()][ksplit == 8 ? 3 : ksplit / 2][per_sm];
+    std::atomic<int>& slot = cache[dev][ksplit == 8 ? 3 : ksplit / 2][per_sm];
     int n = slot.load(std::memory_order_relaxed);
     if (n > 0) return n;
     constexpr auto kern = tb200::ternary_gemv_kernel<MR, WORDS, Epi>;
@@ -453,6 +453,7 @@ template <int MR, typename Epi>
 GemvPlan plan_gemv_fused(int M, int K, int N) {
     const Options& o = options();
     if (o.gemv_words || o.gemv_split) return plan_gemv(M, K, N);
+    const int dev = current_device(), sms = sm_count();
     GemvPlan best{0, 0, 0};
     double best_time = 1e30;
     for (const int words : {16, 32}) {
@@ -462,9 +463,9 @@ GemvPlan plan_gemv_fused(int M, int K, int N) {
             int krange = (K + ks - 1) / ks;
             krange = (krange + stage_rows - 1) / stage_rows * stage_rows;
             if (krange * 4 > tb200::kGemvMaxASlice || (ks > 1 && static_cast<long>(krange) * (ks - 1) >= K)) continue;
-            const int held = words == 16 ? gemv_clusters<MR, 16, Epi>(ks, krange) : gemv_clusters<MR, 32, Epi>(ks, krange);
+            const int held = words == 16 ? gemv_clusters<MR, 16, Epi>(dev, ks, krange) : gemv_clusters<MR, 32, Epi>(dev, ks, krange);
             if (held <= 0) continue;
-            const long shared = (std::min<long>(tiles, held) * ks + sm_count() - 1) / sm_count();          // CTAs of an SM
+            const long shared = (std::min<long>(tiles, held) * ks + sms - 1) / sms;          // CTAs of an SM
             const double row = (shared > 1 ? 2.75e-3 : 3.0e-3) * words / 16;
             const double t = static_cast<double>((tiles + held - 1) / held) * (2.2 + static_cast<double>(shared) * krange * row);
             if (t < best_time) { best_time = t; best = {words, ks, krange}; }
@@ -1368,9 +1369,9 @@ int launch_gemm_split_t(const int8_t* dA, const uint8_t* dW, int M, int K, int N
 }
 // Clusters of the cut form that the device holds at once (asked once per device and form).
 template <int TA, typename Epi>
-int split_clusters(int cut) {
+int split_clusters(int dev, int cut) {
     static std::atomic<int> cache[kMaxDevices][tb200::kSpMaxCut] = {};
-    std::atomic<int>& slot = cache[current_device()][cut - 1];
+    std::atomic<int>& slot = cache[dev][cut - 1];
     int n = slot.load(std::memory_order_relaxed);
     if (n > 0) return n;
     constexpr auto kern = tb200::ternary_gemm_split_kernel<TA, Epi>;
@@ -1404,7 +1405,7 @@ struct SplitPlan {
 template <typename Epi>
 SplitPlan plan_split(int M, int K, int N) {
     const Options& o = options();
-    const int blocks = (K + tb200::kTc3BK - 1) / tb200::kTc3BK;
+    const int blocks = (K + tb200::kTc3BK - 1) / tb200::kTc3BK, dev = current_device();
     if (o.split_rows == 1) return {0, 1};
     if (o.split_rows == 64 || o.split_rows == 128 || o.split_rows == 256)
         return {o.split_rows, std::max(1, std::min({o.split_cut, blocks, tb200::kSpMaxCut}))};
@@ -1416,7 +1417,7 @@ SplitPlan plan_split(int M, int K, int N) {
         const long tiles = (M + rows - 1L) / rows * w_tiles;
         for (int cut = 1; cut <= tb200::kSpMaxCut; ++cut) {
             if (cut > blocks) continue;
-            const int held = rows == 64 ? split_clusters<64, Epi>(cut) : rows == 128 ? split_clusters<128, Epi>(cut) : split_clusters<256, Epi>(cut);
+            const int held = rows == 64 ? split_clusters<64, Epi>(dev, cut) : rows == 128 ? split_clusters<128, Epi>(dev, cut) : split_clusters<256, Epi>(dev, cut);
             if (held <= 0) continue;
             // uncut, a pair writes and finishes the whole tile; with the cut the sum over the pairs grows
             static constexpr double kFixed[3][tb200::kSpMaxCut] = {{5.3, 5.3, 5.45, 5.9}, {7.2, 6.5, 6.6, 6.9}, {9.9, 8.2, 8.3, 8.6}};
