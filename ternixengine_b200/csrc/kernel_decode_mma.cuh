@@ -160,9 +160,15 @@ ternary_decode_mma_kernel(const __grid_constant__ MmaProblem single, const MmaSi
         if (lane == 0) {
             uint32_t t = 0;
             bool ok = true;
+            const MmaProblem* acquired = nullptr;
             for (int i = item_lo; ok && i < item_hi; i += item_step) {
                 const MmaItem it = kSingle ? mma_single_item(sg, i) : items[i];
                 const MmaProblem* p = kSingle ? &single : probs + it.problem;
+                if (!kSingle && p != acquired) {
+                    acquired = p;
+                    tma_acquire_desc(&p->tmap_w);
+                    tma_acquire_desc(&p->tmap_a);
+                }
                 const int tile0 = it.span & 0xffff;
                 const int ntiles = mma_item_tiles(it, p->K);
                 const int row0 = it.row0 & 0xffff;

@@ -255,8 +255,14 @@ ternary_gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             }
             uint32_t it = 0;
             bool ok = true;
+            const CUtensorMap* acquired = nullptr;
             auto walk = make_walk();
             while (ok && walk.next()) {
+                if (kGrouped && walk.ta != acquired) {
+                    acquired = walk.ta;
+                    tma_acquire_desc(walk.ta);
+                    tma_acquire_desc(walk.tw);
+                }
                 const int row0 = walk.m_t * 2 * kTcBM + rank * kTcBM;
                 const int wp_x = walk.n_t * (kTc2TileN / 4) + rank * G::kWpRowBytes;
                 for (int kb = 0; kb < walk.k_blocks; ++kb, ++it) {

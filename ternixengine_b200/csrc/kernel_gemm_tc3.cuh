@@ -227,19 +227,24 @@ struct Tc3Walk {
     const Tc2Tile* tiles;
     int idx, end;
 
-    // (grouped) ask the TMA unit to fetch the operand descriptors of the tile that next() will return
-    __device__ __forceinline__ void prefetch_next_maps() const {
-        if (idx < end) {
-            const Tc3Problem* p = probs + tiles[idx].problem;
-            tma_prefetch_desc(&p->tmap_a);
-            tma_prefetch_desc(&p->tmap_w);
-        }
+    // (grouped) ask the TMA unit to fetch the caller's descriptor of the tile that next() will return, if it is another
+    // problem's than the last one asked for
+    const Tc3Problem* acquired;
+    __device__ __forceinline__ void fetch_next_map(CUtensorMap Tc3Problem::*map) {
+        if (idx >= end) return;
+        const Tc3Problem* p = probs + tiles[idx].problem;
+        if (p == acquired) return;
+        acquired = p;
+        tma_acquire_desc(&(p->*map));
+        tma_prefetch_desc(&(p->*map));
     }
-    __device__ __forceinline__ void prefetch_next_store_map() const {
-        if (idx < end) {
-            const Tc3Problem* p = probs + tiles[idx].problem;
-            if (p->stores.count > 0) tma_prefetch_desc(&p->stores.tmap_c[0]);
-        }
+    __device__ __forceinline__ void fetch_next_store_map() {
+        if (idx >= end) return;
+        const Tc3Problem* p = probs + tiles[idx].problem;
+        if (p == acquired || p->stores.count == 0) return;
+        acquired = p;
+        for (int d = 0; d < p->stores.count; ++d) tma_acquire_desc(&p->stores.tmap_c[d]);
+        tma_prefetch_desc(&p->stores.tmap_c[0]);
     }
     __device__ __forceinline__ bool next() {
         if constexpr (kGrouped) {
@@ -374,12 +379,12 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                 tma_prefetch_desc(&tmap_a);
                 tma_prefetch_desc(&tmap_w);
             } else {
-                w.prefetch_next_maps();
+                w.fetch_next_map(&Tc3Problem::tmap_a);
             }
             while (ok && w.next()) {
-                // the descriptors of the tile after this one: fetched while this tile's loads are issued, so that a
-                // change of problem does not stall the ring for the latency of two descriptor reads
-                if constexpr (kGrouped) w.prefetch_next_maps();
+                // the descriptor of the tile after this one: acquired and fetched while this tile's loads are issued, so that a
+                // change of problem does not stall the ring for the latency of a descriptor read
+                if constexpr (kGrouped) w.fetch_next_map(&Tc3Problem::tmap_a);
                 const int row0 = w.a_t * TA + rank * kRowsPerCta;
                 for (int kb = 0; kb < w.k_blocks; ++kb, ++it) {
                     const uint32_t s = it % S;
@@ -433,10 +438,10 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
             uint32_t it = 0;
             bool ok = true;
             Tc3Walk<kGrouped> w = make_walk();
-            if constexpr (kGrouped) w.prefetch_next_maps();
+            if constexpr (kGrouped) w.fetch_next_map(&Tc3Problem::tmap_w);
             else tma_prefetch_desc(&tmap_w);
             while (ok && w.next()) {
-                if constexpr (kGrouped) w.prefetch_next_maps();
+                if constexpr (kGrouped) w.fetch_next_map(&Tc3Problem::tmap_w);
                 const int wp_x = (w.w_t * kTc3TileW + rank * 128) / 4;
                 for (int kb = 0; kb < w.k_blocks; ++kb, ++it) {
                     const uint32_t sw = it % WS;
@@ -538,11 +543,11 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
         bool ok = true;
         Tc3Walk<kGrouped> w = make_walk();
         if constexpr (kGrouped) {
-            if (elected) w.prefetch_next_store_map();
+            if (elected) w.fetch_next_store_map();
         }
         for (; ok && w.next(); ++lt) {
             if constexpr (kGrouped) {
-                if (elected) w.prefetch_next_store_map();
+                if (elected) w.fetch_next_store_map();
             }
             const int a_t = w.a_t;
             const Tc3Stores* dst = w.st;

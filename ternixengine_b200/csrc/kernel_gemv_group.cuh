@@ -158,6 +158,7 @@ ternary_gemv_group_kernel(const GroupProblem* __restrict__ probs, const GroupIte
         if (lane == 0) {
             uint32_t t = 0;
             bool ok = true;
+            const GroupProblem* acquired = nullptr;
             auto load_tile = [&](const GroupProblem* p, const GroupItem& it, int tt) {
                 const uint32_t s = t % kGroupStages;
                 if (!mbar_wait(&empty[s], ((t / kGroupStages) & 1) ^ 1, abort_flag)) return false;
@@ -175,6 +176,7 @@ ternary_gemv_group_kernel(const GroupProblem* __restrict__ probs, const GroupIte
                 const GroupProblem* p = probs + it.problem;
                 const int K = p->K;
                 const uint32_t n = i - item_lo, buf = n & 1;
+                if (p != acquired) tma_acquire_desc(&(acquired = p)->tmap_w);
                 int rows = p->M - it.row0;
                 if (rows > MR) rows = MR;
                 const int ntiles = (K + kGroupStageRows - 1) / kGroupStageRows;

@@ -305,8 +305,10 @@ ternary_skinny_tc_kernel(const __grid_constant__ SkProblem single, const SkSingl
             if constexpr (!kGrouped) tma_prefetch_desc(&single.tmap_w);
             uint32_t it = 0;
             bool ok = true;
+            const SkProblem* acquired = nullptr;
             SkWalk<kGrouped> w = make_walk();
             while (ok && w.next()) {
+                if (kGrouped && w.p != acquired) tma_acquire_desc(&(acquired = w.p)->tmap_w);
                 const int x = w.block * kSkWpRowBytes;
                 for (int s = w.s0; s < w.s1; ++s, ++it) {
                     const uint32_t sl = it % WS;
@@ -326,8 +328,10 @@ ternary_skinny_tc_kernel(const __grid_constant__ SkProblem single, const SkSingl
             if constexpr (!kGrouped) tma_prefetch_desc(&single.tmap_a);
             uint32_t it = 0;
             bool ok = true;
+            const SkProblem* acquired = nullptr;
             SkWalk<kGrouped> w = make_walk();
             while (ok && w.next()) {
+                if (kGrouped && w.p != acquired) tma_acquire_desc(&(acquired = w.p)->tmap_a);
                 for (int s = w.s0; s < w.s1; ++s, ++it) {
                     const uint32_t sl = it % AS;
                     if (!mbar_wait_backoff(&a_empty[sl], ((it / AS) & 1) ^ 1, abort_flag, 32)) { ok = false; break; }

@@ -129,6 +129,13 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 __device__ __forceinline__ void tma_prefetch_desc(const void* tmap) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
 }
+// A descriptor that lies in global memory (the tables of a problem group, which the host copies there) is read through a
+// proxy with a cache of its own, which ordinary writes to that memory do not reach: a new table at the address of an old
+// one, or a table copied over, could be met with the old descriptors.  So every CTA acquires a descriptor before its first
+// use of it, prefetches included (.sys: the host wrote it).  Descriptors passed as kernel parameters need none of this.
+__device__ __forceinline__ void tma_acquire_desc(const void* tmap) {
+    asm volatile("fence.proxy.tensormap::generic.acquire.sys [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
+}
 // x = innermost coordinate (its byte offset must be a multiple of 16), y = row.
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tmap, int x, int y, uint64_t* bar) {
     asm volatile(
