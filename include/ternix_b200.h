@@ -54,6 +54,9 @@ extern "C" {
 #define TERNIX_B200_LAUNCHED_GEMM_TC3    7  /* paired CTAs, weights decoded into tensor memory             */
 #define TERNIX_B200_LAUNCHED_GEMM_SPLIT  8  /* the same, K cut between the pairs of a cluster (fused epilogue only) */
 
+/* Largest M, K or N that an entry point takes (2^31 - 1025); beyond it, as for negative sizes, TERNIX_B200_ERR_INVALID_SHAPE. */
+#define TERNIX_B200_MAX_SIZE 2147482623
+
 const char *ternix_b200_status_string(int status);
 /* cudaError_t (as int) of the last failing CUDA call made by the calling thread, 0 if none. */
 int ternix_b200_last_cuda_error(void);

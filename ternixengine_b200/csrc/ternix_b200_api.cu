@@ -44,6 +44,13 @@ int cuda_fail(cudaError_t e) {
         if (e_ != cudaSuccess) return cuda_fail(e_);             \
     } while (0)
 
+// Whether every size is one that the entry points take.  The room up to 2^31 is for index arithmetic in int: tiles and slabs
+// round sizes up, and a loop's index passes the size by one step, at most 1024, before it ends.
+template <typename... Sizes>
+bool sizes_ok(Sizes... sizes) {
+    return ((sizes >= 0 && sizes <= TERNIX_B200_MAX_SIZE) && ...);
+}
+
 // The scaled accumulators of the fast kernels hold 64 * sum; 64 * 128 * K must stay below 2^31.
 constexpr int kMaxScaledK = 262143;
 
@@ -1757,7 +1764,7 @@ int ternix_b200_release_cached_memory(void) {
 int ternix_b200_select_kernel(const void* dA, const void* dW, const void* dC, int M, int K, int N, long long ldc) {
     (void)dC;
     (void)ldc;
-    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return -TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K, N) || (N % 4) != 0) return -TERNIX_B200_ERR_INVALID_SHAPE;
     return select_kernel(dA, dW, M, K, N);
 }
 
@@ -1765,7 +1772,7 @@ int ternix_b200_matmul_ex(const int8_t* dA, const uint8_t* dW, int32_t* dC, int 
                           int kernel, int32_t* d_status, void* stream) {
     // Shape first, before any pointer is looked at (the reference's wrappers promise the same,
     // tests/test_cuda_matmul.cu:41-43).
-    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (ldc < N) return TERNIX_B200_ERR_INVALID_ARG;
     if (kernel < TERNIX_B200_KERNEL_AUTO || kernel > TERNIX_B200_KERNEL_SKINNY_TC) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0 || N == 0) return TERNIX_B200_OK;
@@ -1977,7 +1984,7 @@ int host_slab_plan(int M, int K, int N, bool* by_rows) {
 extern "C" {
 
 int ternix_b200_matmul_host(const int8_t* A, const uint8_t* Wp, int32_t* C, int M, int K, int N, int kernel) {
-    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (kernel < TERNIX_B200_KERNEL_AUTO || kernel > TERNIX_B200_KERNEL_SKINNY_TC) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0 || N == 0) return TERNIX_B200_OK;
     if (!C || (K > 0 && (!A || !Wp))) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2043,7 +2050,7 @@ int ternix_b200_shard_columns(int N, int world, int rank, int granule, int* n0, 
 
 int ternix_b200_unpack_gathered(const int32_t* d_gathered, int32_t* dC, int M, int N, long long ldc, int world,
                                 int granule, int n_pad, void* stream) {
-    if (M < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (world < 1 || granule < 4 || (granule % 4) != 0 || ldc < N || n_pad < 0) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0 || N == 0) return TERNIX_B200_OK;
     if (!d_gathered || !dC) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2064,7 +2071,7 @@ static int group_create_impl(ternix_b200_group** out, const ternix_b200_problem*
     *out = nullptr;
     for (int i = 0; i < count; ++i) {
         const ternix_b200_problem& q = problems[i];
-        if (q.M < 0 || q.K < 0 || q.N < 0 || (q.N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+        if (!sizes_ok(q.M, q.K, q.N) || (q.N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
         if (q.ldc < q.N) return TERNIX_B200_ERR_INVALID_ARG;
         if (q.M > 0 && q.N > 0 && (!q.dC || (q.K > 0 && (!q.dA || !q.dW)))) return TERNIX_B200_ERR_INVALID_ARG;
     }
@@ -2398,12 +2405,12 @@ int ternix_b200_group_create_prepacked(ternix_b200_group** out, const ternix_b20
 }
 
 size_t ternix_b200_prepack_k4_bytes(int K, int N) {
-    if (K < 0 || N < 0 || (N % 4) != 0) return 0;
+    if (!sizes_ok(K, N) || (N % 4) != 0) return 0;
     return static_cast<size_t>((K + 3) / 4) * static_cast<size_t>(N);
 }
 
 int ternix_b200_prepack_k4(const uint8_t* dW, uint8_t* dW_prepacked, int K, int N, void* stream) {
-    if (K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (K == 0 || N == 0) return TERNIX_B200_OK;
     if (!dW || !dW_prepacked || !aligned(dW_prepacked, 16)) return TERNIX_B200_ERR_INVALID_ARG;
     const long long total = static_cast<long long>((K + 3) / 4) * (N / 4);
@@ -2502,7 +2509,7 @@ void ternix_b200_group_destroy(ternix_b200_group* g) {
 
 int ternix_b200_matmul_bcast(const int8_t* dA, const uint8_t* dW, int32_t* const* dC_list, int n_dest, int M, int K,
                              int N, long long ldc, int32_t* d_status, void* stream) {
-    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (ldc < N || n_dest < 1 || n_dest > tb200::kTc2MaxDest || !dC_list) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0 || N == 0) return TERNIX_B200_OK;
     for (int d = 0; d < n_dest; ++d)
@@ -2553,7 +2560,7 @@ int ternix_b200_gemv_batch_noalloc(const ternix_b200_problem* problems, int coun
     if (count > kNoAllocMaxProblems) return TERNIX_B200_ERR_TOO_LARGE;
     for (int i = 0; i < count; ++i) {
         const ternix_b200_problem& q = problems[i];
-        if (q.M < 0 || q.K < 0 || q.N < 0 || (q.N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+        if (!sizes_ok(q.M, q.K, q.N) || (q.N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
         if (q.ldc < q.N) return TERNIX_B200_ERR_INVALID_ARG;
         if (q.M == 0 || q.N == 0) continue;
         if (!q.dC || (q.K > 0 && (!q.dA || !q.dW))) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2655,7 +2662,7 @@ int ternix_b200_gemv_batch_noalloc_limits(int* max_problems, int* max_items, lon
 int ternix_b200_weights_create(ternix_b200_weights** out, const uint8_t* dW, int K, int N) {
     if (!out) return TERNIX_B200_ERR_INVALID_ARG;
     *out = nullptr;
-    if (K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (K > 0 && N > 0 && !dW) return TERNIX_B200_ERR_INVALID_ARG;
     ternix_b200_weights* w = new (std::nothrow) ternix_b200_weights();
     if (!w) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2676,7 +2683,7 @@ int ternix_b200_weights_create(ternix_b200_weights** out, const uint8_t* dW, int
 
 int ternix_b200_weights_matmul_host(ternix_b200_weights* w, const int8_t* A, int32_t* C, int M) {
     if (!w) return TERNIX_B200_ERR_INVALID_ARG;
-    if (M < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M)) return TERNIX_B200_ERR_INVALID_SHAPE;
     const int K = w->K, N = w->N;
     if (M == 0 || N == 0) return TERNIX_B200_OK;
     if (!C || (K > 0 && !A)) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2695,7 +2702,7 @@ void ternix_b200_weights_destroy(ternix_b200_weights* w) { delete w; }
 int ternix_b200_weights_matmul(ternix_b200_weights* w, const int8_t* dA, int32_t* dC, int M, long long ldc,
                                int32_t* d_status, void* stream) {
     if (!w) return TERNIX_B200_ERR_INVALID_ARG;
-    if (M < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M)) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (ldc < w->N) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0 || w->N == 0) return TERNIX_B200_OK;
     const int K = w->K, N = w->N;
@@ -2790,7 +2797,7 @@ int ternix_b200_pack_ternary_device(uint8_t* d_packed, const int8_t* d_unpacked,
 
 int ternix_b200_quantize_rows(const void* dX, int x_dtype, long long ldx, int8_t* dA, float* d_row_scale, int M, int K,
                               void* stream) {
-    if (M < 0 || K < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K)) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (x_dtype != TERNIX_B200_DTYPE_F32 && x_dtype != TERNIX_B200_DTYPE_BF16) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0) return TERNIX_B200_OK;
     if (!dX || !dA || !d_row_scale || ldx < K) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2806,7 +2813,7 @@ int ternix_b200_quantize_rows(const void* dX, int x_dtype, long long ldx, int8_t
 int ternix_b200_rmsnorm_quantize(const void* dX, long long ldx, const void* dResidual, long long ldr, int x_dtype,
                                  const void* dWeight, int w_dtype, float eps, void* dH, long long ldh, int8_t* dA,
                                  float* d_row_scale, int M, int K, void* stream) {
-    if (M < 0 || K < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K)) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (!dtype_ok(x_dtype) || (dWeight && w_dtype != x_dtype && w_dtype != TERNIX_B200_DTYPE_F32)) return TERNIX_B200_ERR_INVALID_ARG;
     if (!(eps >= 1e-12f && eps <= 1.0f)) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0) return TERNIX_B200_OK;
@@ -2825,7 +2832,7 @@ int ternix_b200_rmsnorm_quantize(const void* dX, long long ldx, const void* dRes
 int ternix_b200_glu_quantize(const void* dGate, long long ldg, const void* dUp, long long ldu, int dtype, int activation,
                              int norm, const void* dWeight, int w_dtype, float eps, int8_t* dA, float* d_row_scale, int M,
                              int K, void* stream) {
-    if (M < 0 || K < 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K)) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (!dtype_ok(dtype) || !activation_ok(activation)) return TERNIX_B200_ERR_INVALID_ARG;
     if (dWeight && (!norm || (w_dtype != dtype && w_dtype != TERNIX_B200_DTYPE_F32))) return TERNIX_B200_ERR_INVALID_ARG;
     if (norm && !(eps >= 1e-12f && eps <= 1.0f)) return TERNIX_B200_ERR_INVALID_ARG;
@@ -2841,7 +2848,7 @@ int ternix_b200_glu_quantize(const void* dGate, long long ldg, const void* dUp, 
 
 int ternix_b200_matmul_fused(const int8_t* dA, const uint8_t* dW, const ternix_b200_epilogue* ep, void* dY, long long ldy,
                              int M, int K, int N, int kernel, int32_t* d_status, void* stream) {
-    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (!ep || ldy < N || !dtype_ok(ep->out_dtype) || !activation_ok(ep->activation)) return TERNIX_B200_ERR_INVALID_ARG;
     if (kernel < TERNIX_B200_KERNEL_AUTO || kernel > TERNIX_B200_KERNEL_SKINNY_TC) return TERNIX_B200_ERR_INVALID_ARG;
     if (ep->bias && (!dtype_ok(ep->bias_dtype) || !aligned(ep->bias, static_cast<uintptr_t>(dtype_bytes(ep->bias_dtype)))))
@@ -2875,7 +2882,7 @@ int ternix_b200_matmul_fused(const int8_t* dA, const uint8_t* dW, const ternix_b
 int ternix_b200_matmul_dequant(const int8_t* dA, const uint8_t* dW, void* const* dY_list, int n_dest,
                                const float* d_row_scale, float w_scale, int M, int K, int N, long long ldy,
                                int32_t* d_status, void* stream) {
-    if (M < 0 || K < 0 || N < 0 || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
+    if (!sizes_ok(M, K, N) || (N % 4) != 0) return TERNIX_B200_ERR_INVALID_SHAPE;
     if (ldy < N || n_dest < 1 || n_dest > tb200::kTc2MaxDest || !dY_list || !d_row_scale) return TERNIX_B200_ERR_INVALID_ARG;
     if (M == 0 || N == 0) return TERNIX_B200_OK;
     for (int d = 0; d < n_dest; ++d)

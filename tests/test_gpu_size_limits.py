@@ -1,0 +1,21 @@
+"""The longest row that the layer operators take."""
+import numpy as np
+import pytest
+
+import ternixengine_b200 as tb
+
+pytestmark = pytest.mark.gpu
+
+
+def test_longest_row():
+    """2^31 - 1025 columns (4.3 GB of bfloat16): every index of the row, and the step that ends its loops, in a C int."""
+    import torch
+    K = 2 ** 31 - 1025
+    x = torch.zeros((1, K), dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, 1023, 2 ** 30, K - 1025, K - 2, K - 1]
+    x[0, at] = torch.tensor([1, -2, 3, 127, -4, 5, -127], dtype=torch.bfloat16, device="cuda")
+    codes, scale = tb.rmsnorm_quantize(x, eps=1e-5)
+    assert codes[0, at].tolist() == [1, -2, 3, 127, -4, 5, -127] and int(torch.count_nonzero(codes)) == len(at)
+    ms = (1 + 4 + 9 + 127 ** 2 + 16 + 25 + 127 ** 2) / K
+    # every partial sum is a whole number below 2^24, so the sum is exact: division, addition, root, reciprocal and product round once each, and 127 / 127
+    assert abs(float(scale) - 1 / np.sqrt(ms + float(np.float32(1e-5)))) <= 6 * 2.0 ** -24 * float(scale)
