@@ -286,9 +286,9 @@ bool gemm_tc_ok(const void* dA, const void* dW, int K, int N) {
 // against 97 us here, 16 rows 732 us against 148 us.
 constexpr int kGroupMmaMinRows = 2, kGroupMmaMaxRows = 64;
 
-// Batched decode on the warp-level tensor instruction: row groups of 8 or 16, any M >= 1.
+// Batched decode on the warp-level tensor instruction: row groups of 8 or 16; a work item holds its first row in 16 bits.
 bool decode_mma_ok(const void* dA, const void* dW, int M, int K, int N) {
-    return M >= 1 && (N % 64) == 0 && (K % 16) == 0 && K >= 16 && K <= 65536 && aligned(dA, 16) && aligned(dW, 16);
+    return M >= 1 && M <= 65536 && (N % 64) == 0 && (K % 16) == 0 && K >= 16 && K <= 65536 && aligned(dA, 16) && aligned(dW, 16);
 }
 // Tensor-memory decode kernel (kernel_skinny_tc.cuh): up to 128 rows.
 bool skinny_ok(const void* dA, const void* dW, int M, int K, int N) {

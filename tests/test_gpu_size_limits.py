@@ -19,3 +19,13 @@ def test_longest_row():
     ms = (1 + 4 + 9 + 127 ** 2 + 16 + 25 + 127 ** 2) / K
     # every partial sum is a whole number below 2^24, so the sum is exact: division, addition, root, reciprocal and product round once each, and 127 / 127
     assert abs(float(scale) - 1 / np.sqrt(ms + float(np.float32(1e-5)))) <= 6 * 2.0 ** -24 * float(scale)
+
+
+def test_most_rows_of_the_mma_sync_kernel():
+    import torch
+    M, K, N = 65536, 64, 128
+    a = torch.randint(-127, 128, (M, K), dtype=torch.int8, device="cuda")
+    w = torch.from_numpy(tb.synth_packed_weights(K, N, 1)).cuda()
+    rs = torch.rand(M, device="cuda")
+    assert torch.equal(tb.matmul(a, w, kernel="decode_mma"), tb.matmul(a, w, kernel="generic"))
+    assert torch.equal(tb.matmul_fused(a, w, rs, 0.5, kernel="decode_mma"), tb.matmul_fused(a, w, rs, 0.5, kernel="generic"))

@@ -39,3 +39,11 @@ def test_products(n):
 def test_nothing_to_do_stays_nothing():
     assert tb.lib.ternix_b200_rmsnorm_quantize(None, MAX, None, 0, 1, None, 0, 1e-5, None, 0, None, None, 0, MAX, None) == tb.OK
     assert tb.lib.ternix_b200_matmul_ex(None, None, None, 0, MAX, 4, 4, 0, None, None) == tb.OK
+
+
+def test_rows_of_the_mma_sync_kernel():
+    """Its work items hold a row in 16 bits: row 65536 would be row 0 again."""
+    ep = tb._Epilogue(row_scale=P, w_scale=1.0, out_dtype=1)
+    for M in (65537, 70000):
+        assert tb.lib.ternix_b200_matmul_fused(P, P, ctypes.byref(ep), P, 64, M, 64, 64, tb.KERNEL_DECODE_MMA, None, None) == tb.ERR_UNSUPPORTED
+        assert tb.lib.ternix_b200_matmul_ex(P, P, P, M, 64, 64, 64, tb.KERNEL_DECODE_MMA, None, None) == tb.ERR_UNSUPPORTED
