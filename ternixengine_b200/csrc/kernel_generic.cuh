@@ -121,7 +121,9 @@ ternary_generic_fused_kernel(const int8_t* A, const uint8_t* W, int M, int K, in
 
     const int tid = threadIdx.x, tx = tid & 31, ty = tid >> 5;
     const int pitch = N >> 2;
-    const int row0 = blockIdx.y * kGenRows, byte0 = blockIdx.x * kGenBytes;
+    // tiles numbered along x only, columns fastest: the grid's y would end at 65535 row tiles
+    const int tiles_x = (pitch + kGenBytes - 1) / kGenBytes;
+    const int row0 = static_cast<int>(blockIdx.x) / tiles_x * kGenRows, byte0 = static_cast<int>(blockIdx.x) % tiles_x * kGenBytes;
     dependent_wait();
 
     int32_t acc[4][4] = {}, total[4][4] = {};

@@ -1356,9 +1356,9 @@ int launch_row_quant_dtype(int dtype, const tb200::RowQuantArgs& p, cudaStream_t
 // ---------------------------------------------------------------- the product with the fused epilogue (epilogue.cuh)
 template <typename Epi>
 int launch_generic_fused(const int8_t* dA, const uint8_t* dW, int M, int K, int N, const Epi& epi, cudaStream_t st) {
-    dim3 grid((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes, (M + tb200::kGenRows - 1) / tb200::kGenRows);
-    if (grid.y > 65535) return TERNIX_B200_ERR_INVALID_SHAPE;
-    return launch_layer(tb200::ternary_generic_fused_kernel<Epi>, grid, tb200::kGenThreads, 0, 1, st, dA, dW, M, K, N, epi);
+    const long long tiles = static_cast<long long>((N / 4 + tb200::kGenBytes - 1) / tb200::kGenBytes) * ((M + tb200::kGenRows - 1) / tb200::kGenRows);
+    if (tiles > 0x7fffffff) return TERNIX_B200_ERR_INVALID_SHAPE;
+    return launch_layer(tb200::ternary_generic_fused_kernel<Epi>, dim3(static_cast<unsigned>(tiles)), tb200::kGenThreads, 0, 1, st, dA, dW, M, K, N, epi);
 }
 
 // The cut prefill form (kernel_gemm_split.cuh): tile rows, and pairs that share a tile's K.

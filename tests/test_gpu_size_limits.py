@@ -29,3 +29,17 @@ def test_most_rows_of_the_mma_sync_kernel():
     rs = torch.rand(M, device="cuda")
     assert torch.equal(tb.matmul(a, w, kernel="decode_mma"), tb.matmul(a, w, kernel="generic"))
     assert torch.equal(tb.matmul_fused(a, w, rs, 0.5, kernel="decode_mma"), tb.matmul_fused(a, w, rs, 0.5, kernel="generic"))
+
+
+@pytest.mark.parametrize("K", [0, 3])
+def test_more_rows_than_65535_tiles_of_the_generic_kernel(K):
+    """K = 0 (nothing but the epilogue is left) and a forced kernel, at rows beyond 65535 x 32."""
+    import torch
+    M, N = 65535 * 32 + 37, 132
+    a = torch.randint(-127, 128, (M, K), dtype=torch.int8, device="cuda")
+    wp = tb.synth_packed_weights(K, N, 1) if K else np.zeros((0, N // 4), dtype=np.uint8)
+    w = torch.from_numpy(tb.unpack_ternary(wp)).cuda().float()
+    rs, bias = torch.full((M,), 0.5, device="cuda"), torch.arange(N, device="cuda").float()
+    y = tb.matmul_fused(a, torch.from_numpy(wp).cuda(), rs, 1.0, bias=bias, out_dtype=torch.float32, kernel="auto" if K == 0 else "generic")
+    for rows in (slice(0, 70), slice(65535 * 32 - 40, M)):
+        assert torch.equal(y[rows], (a[rows].float() @ w) * 0.5 + bias)           # halves of small whole numbers: exact
