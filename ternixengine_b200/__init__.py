@@ -168,6 +168,16 @@ def _check(status: int, where: str) -> None:
     raise TernixError(status, msg)
 
 
+MAX_SIZE = 2147482623          # TERNIX_B200_MAX_SIZE
+
+
+def _sizes(*sizes) -> None:
+    """Refuses sizes that the C ABI does not take; ctypes would hand on the low 32 bits of a larger one."""
+    for n in sizes:
+        if n > MAX_SIZE:
+            raise ValueError(f"sizes go up to {MAX_SIZE}, not {n}")
+
+
 def set_option(name: str, value=None) -> None:
     """Sets a tuning option of the library (ternix_b200_set_option); value None restores the default."""
     v = None if value is None else str(value).encode()
@@ -235,6 +245,7 @@ def ternary_matmul_host(a: np.ndarray, b_packed: np.ndarray, kernel: str = "auto
     if b_packed.shape[0] != K:
         raise ValueError("inner dimensions do not match")
     N = b_packed.shape[1] * 4
+    _sizes(M, K, N)
     c = np.empty((M, N), dtype=np.int32)
     _check(lib.ternix_b200_matmul_host(_np_ptr(a), _np_ptr(b_packed), _np_ptr(c), M, K, N, KERNELS[kernel]),
            "ternary_matmul_host")
@@ -286,6 +297,7 @@ def matmul(a, w_packed, out=None, kernel: str = "auto", status=None, stream=None
     if w_packed.shape[0] != K:
         raise ValueError("inner dimensions do not match")
     N = w_packed.shape[1] * 4
+    _sizes(M, K, N)
     if out is None:
         out = torch.empty((M, N), dtype=torch.int32, device=a.device)
     if out.dtype != torch.int32 or tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1):
@@ -311,6 +323,7 @@ class TernaryWeights:
             raise ValueError("TernaryWeights takes a contiguous CUDA uint8 (K, N/4) tensor")
         self.w = w_packed
         self.K, self.N = w_packed.shape[0], w_packed.shape[1] * 4
+        _sizes(self.K, self.N)
         h = ctypes.c_void_p()
         with torch.cuda.device(w_packed.device):
             _check(lib.ternix_b200_weights_create(ctypes.byref(h), w_packed.data_ptr(), self.K, self.N), "weights_create")
@@ -322,6 +335,7 @@ class TernaryWeights:
         if not a.is_cuda or a.dtype != torch.int8 or a.dim() != 2 or not a.is_contiguous() or a.shape[1] != self.K:
             raise ValueError("A must be a contiguous CUDA int8 (M, K) tensor")
         M = a.shape[0]
+        _sizes(M)
         if out is None:
             out = torch.empty((M, self.N), dtype=torch.int32, device=a.device)
         if out.dtype != torch.int32 or tuple(out.shape) != (M, self.N) or (self.N > 1 and out.stride(1) != 1):
@@ -350,6 +364,7 @@ class TernaryWeights:
             return x.data_ptr()
 
         M = a_host.shape[0]
+        _sizes(M)
         if out_host is None:
             out_host = torch.empty((M, self.N), dtype=torch.int32, pin_memory=True)
         pa = host_ptr(a_host, np.int8, torch.int8, (M, self.K), "A")
@@ -388,6 +403,7 @@ def quantize_rows(x):
     if not x.is_cuda or x.dim() != 2 or x.stride(1) != 1 or x.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("quantize_rows takes a CUDA float32 or bfloat16 (M, K) tensor with unit column stride")
     M, K = x.shape
+    _sizes(M, K)
     a = torch.empty((M, K), dtype=torch.int8, device=x.device)
     scale = torch.empty((M,), dtype=torch.float32, device=x.device)
     with torch.cuda.device(x.device):
@@ -403,6 +419,7 @@ def matmul_dequant(a, w_packed, row_scale, w_scale: float, out=None, status=None
 
     M, K = a.shape
     N = w_packed.shape[1] * 4
+    _sizes(M, K, N)
     if out is None:
         out = torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
     if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N) or out.stride(1) != 1:
@@ -504,6 +521,7 @@ def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None,
     code, dev, shape = rt.codes.get(dtype), x.get_device(), x.shape
     if code is None or dev < 0 or len(shape) != 2:
         raise ValueError("rmsnorm_quantize takes a CUDA (M, K) bfloat16, float16 or float32 tensor")
+    _sizes(*shape)
     ldx = _rows(x, "x", dev, dtype, shape)
     M, K = shape
     pr = ph = pw = None
@@ -546,6 +564,7 @@ def glu_quantize(gate, up, activation: str = "silu", weight=None, eps=None, out=
     code, dev, shape = rt.codes.get(dtype), gate.get_device(), gate.shape
     if code is None or dev < 0 or len(shape) != 2:
         raise ValueError("glu_quantize takes CUDA (M, K) bfloat16, float16 or float32 tensors")
+    _sizes(*shape)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
     if weight is not None and eps is None:
@@ -594,6 +613,7 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
     if sw[0] != K:
         raise ValueError("inner dimensions do not match")
     N = sw[1] * 4
+    _sizes(M, K, N)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
     if kern is None:
@@ -655,6 +675,7 @@ class ProjectionGroup:
             if w.shape[0] != ((K + 3) // 4 if prepacked else K) or tuple(out.shape) != (M, N) or \
                     (N > 1 and out.stride(1) != 1):
                 raise ValueError("shape mismatch")
+            _sizes(M, K, N)
             arr[i] = _Problem(a.data_ptr(), w.data_ptr(), out.data_ptr(), M, K, N,
                               out.stride(0) if M > 1 else max(N, out.stride(0)))
             self._keep.append((a, w, out))
@@ -699,6 +720,7 @@ def prepack_k4(w_packed):
     if not w_packed.is_cuda or w_packed.dtype != torch.uint8 or w_packed.dim() != 2 or not w_packed.is_contiguous():
         raise ValueError("prepack_k4 takes a contiguous CUDA uint8 (K, N/4) tensor")
     K, N = w_packed.shape[0], w_packed.shape[1] * 4
+    _sizes(K, N)
     out = torch.empty(((K + 3) // 4, N), dtype=torch.uint8, device=w_packed.device)
     with torch.cuda.device(w_packed.device):
         _check(lib.ternix_b200_prepack_k4(w_packed.data_ptr(), out.data_ptr(), K, N,
@@ -971,6 +993,7 @@ class ShardedTernaryLinear:
         import torch
 
         M = a.shape[0]
+        _sizes(M)
         if self.mode == "local":
             if out is None:
                 out = torch.empty((M, self.N), dtype=torch.int32, device=a.device)

@@ -43,3 +43,15 @@ def test_more_rows_than_65535_tiles_of_the_generic_kernel(K):
     y = tb.matmul_fused(a, torch.from_numpy(wp).cuda(), rs, 1.0, bias=bias, out_dtype=torch.float32, kernel="auto" if K == 0 else "generic")
     for rows in (slice(0, 70), slice(65535 * 32 - 40, M)):
         assert torch.equal(y[rows], (a[rows].float() @ w) * 0.5 + bias)           # halves of small whole numbers: exact
+
+
+def test_sizes_of_more_than_32_bits():
+    """2^32 + 5 rows and 2^32 + 64 columns, which would arrive in a C int as 5 and 64."""
+    import torch
+    x = torch.empty((2 ** 32 + 5, 1), dtype=torch.bfloat16, device="cuda")
+    w = torch.empty((1, 2 ** 30 + 16), dtype=torch.uint8, device="cuda")
+    a, s = torch.ones((1, 1), dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda")
+    for call in (lambda: tb.rmsnorm_quantize(x), lambda: tb.rmsnorm_quantize(x.view(1, -1)), lambda: tb.glu_quantize(x, x), lambda: tb.quantize_rows(x),
+                 lambda: tb.matmul_fused(a, w, s), lambda: tb.matmul(a, w), lambda: tb.matmul_dequant(a, w, s, 1.0), lambda: tb.TernaryWeights(w)):
+        with pytest.raises(ValueError):
+            call()
