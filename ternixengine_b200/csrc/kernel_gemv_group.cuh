@@ -183,9 +183,10 @@ ternary_gemv_group_kernel(const GroupProblem* __restrict__ probs, const GroupIte
                 int tt = 0;
                 if (i == item_lo) {
                     // Launched as a programmatic dependent of the kernel before it, this CTA may already be running
-                    // while that kernel's last CTAs finish.  Weights are never written by a kernel of this library, so
-                    // the first ring of weight tiles is requested right away; everything a predecessor may have
-                    // produced (the activations) and every store waits for its completion.
+                    // while that kernel does.  The first ring of weight tiles is requested right away: only kernels that
+                    // write none of a group's weights let their dependents begin early (see launch_decode_batch), and
+                    // all before them is complete.  Everything such a kernel may have produced (the activations) and
+                    // every store waits for its completion.
                     for (; ok && tt < ntiles && tt < kGroupStages; ++tt) ok = load_tile(p, it, tt);
                     asm volatile("griddepcontrol.wait;" ::: "memory");
                     if (!ok) break;
@@ -206,6 +207,9 @@ ternary_gemv_group_kernel(const GroupProblem* __restrict__ probs, const GroupIte
         }
     } else {
         // ------------------------------------------------------------ consumers
+        // They need the activations first, which come behind the kernel before; met here, its run time does not count
+        // towards the limit of their bounded wait.
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         const int kg = warp;                                   // prepacked: 4-row groups kg and kg + 8 of each stage
         // transposing loads: 128-column block `cb`, 16-row blocks `kb0` and `kb0 + (blocks per stage) / 2`; this lane's
         // row address inside the swizzled stage and its four k-rows inside a block.  128-byte rows: 4 column blocks x

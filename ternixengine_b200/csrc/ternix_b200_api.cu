@@ -1068,11 +1068,20 @@ bool group_gemv_ok(const ternix_b200_problem& q) {
 }
 
 // Launch of the persistent one-row decode kernel.  A short launch (at most four items per CTA) is made a programmatic
-// dependent of the kernel before it on the stream: when that kernel is another decode batch of this library (the
-// only kernels here that release their dependents early), the new grid's CTAs move onto SMs as the old grid's CTAs
-// retire and request their first weight tiles while the old grid finishes; they read activations and write C only
-// after it has completed (griddepcontrol.wait).  Behind any other kernel or copy the launch waits for full completion
-// as usual.  Measured: 64 x config 1 per launch 51.6 -> 48.7 us.  Long launches lose by it (256 x config 1: 182 -> 192
+// dependent of the kernel before it on the stream: when that kernel is another decode batch or a layer kernel of this
+// library (launch_layer), the new grid's CTAs move onto SMs that have room for them and request their first weight tiles
+// while the old grid finishes; they read activations and write C only after it has completed (griddepcontrol.wait).
+// Behind any other kernel or copy the launch waits for full completion as usual.
+//
+// Why weights may be read so early.  Two kinds of kernels here release their dependents before they end.  A layer kernel
+// does so behind its own wait, so whatever came before it is complete; it writes codes, scales, streams and outputs, or (the
+// aligned copy) scratch that only the launch behind it reads.  A decode batch does so at once, in front of its own wait, and
+// writes C; what it follows may thus still run when the batch after it reads weights, but that is again one of these two
+// kinds, or it would not have let the batch begin.  Whatever writes weights (a copy, a packing kernel, any kernel of
+// the caller's) releases nothing early.  In the other direction a layer kernel touches no memory before its wait, which
+// returns when the batch before it has completed, and a batch completes behind its own wait.
+//
+// Measured: 64 x config 1 per launch 51.6 -> 48.7 us.  Long launches lose by it (256 x config 1: 182 -> 192
 // us): CTAs that start one by one no longer walk the same weight rows as their neighbours at the same time, which
 // costs more DRAM efficiency than the filled ramp gains.  Option gemv_pdl = 0 | 1 forces the choice.
 template <class Kern>
