@@ -42,10 +42,11 @@ def activation_error(v, act):
     denominators above 2^126 (documented), where the quotient is at most |v| 2^-126.  gelu = 0.5 v (1 + erf): erff has 2 ulp and its argument
     one rounding and a rounded constant (|d erf| <= 1.13 |x| 2^-23 <= 2^-23 where erf still moves), the sum one rounding of
     a value up to 2: in all |v| (2 x 2^-24 + 2^-23 + 2 x 2^-24) / 2, and two roundings of the products.  The same bound holds for
-    gelu = v / (1 + 2^-w), w the base-2 logit of the normal distribution P from a fit that is level at 1.2e-8 in P: P is off by
-    that, by P (1 - P) <= 1/4 times the exponential's 2^-22 and three roundings of w (P (1 - P) |w| <= 0.23 in natural units, so
-    0.23 x 3 x 2^-24), and by 2^-22 P from sum, reciprocal and product: 1.2e-7 + 2.4e-7 P against 1.8e-7 + 1.2e-7 P here and the
-    2^-24 P that every comparison adds for the result's rounding; where P nears 1 the first term vanishes with 1 - P."""
+    gelu = v / (1 + 2^-w), w the base-2 logit of the normal distribution P from a fit that is off by at most 1.2e-8 in v P(v) and
+    3e-8 in P: P is off by that, by P (1 - P) <= 1/4 times the exponential's 2^-22 and three roundings of w (P (1 - P) |w| <= 0.23
+    in natural units, so 0.23 x 3 x 2^-24), and by 2^-22 P from sum, reciprocal and product: 1.3e-7 + 2.4e-7 P against 1.8e-7 +
+    1.2e-7 P here and the 2^-24 P that every comparison adds for the result's rounding; where P nears 1 the first term vanishes
+    with 1 - P.  (float32 data have smaller errors than these.)"""
     v = np.asarray(v, dtype=np.float64)
     out = np.abs(activate64(v, act))
     if act == "silu":

@@ -55,26 +55,41 @@ __device__ __forceinline__ float logistic_times(float v, float u) {
     return v * rcp_approx(1.0f + exp2_approx(-1.44269504f * u));
 }
 // log2 of P(v) / P(-v) over v, P the normal distribution: v P(v), the exact GELU, is v / (1 + 2^(-that v)).  Odd in v and smooth, so
-// a polynomial in v^2; this one is a least-squares fit in Chebyshev points of v^2 on [0, 32], weighted by P(v) P(-v) and reweighted
-// (Lawson's method) until the error in P is level: 1.2e-8.  Beyond v^2 = 32 it stays constant, where P is within 1e-8 of 0 or 1.
-// P is then off by at most 1.2e-7 (the fit, P (1 - P) times the exponential's 2^-22 and its argument's roundings) and 2^-22 of
-// itself (sum, reciprocal, product), as little as with the library's erf, whose form took 98 us where this one takes 68 (4096 x
-// 2560 x 6912; SiLU 54) and 167 where it takes 124 (gate 4096 x 28672; SiLU 112).
+// a polynomial in v^2; this one is a least-squares fit in Chebyshev points of v^2 on [0, 32], weighted by |v| P(v) P(-v) and
+// reweighted (Lawson's method) until the error in v P(v) is level.  With the coefficients as float32, v P(v) is off by at most
+// 1.2e-8 for every v: beyond v^2 = 32 the logit stays constant, P(-v) goes on falling, and what it is off by is below that too.
 __device__ __forceinline__ float gelu_logit(float v) {
     const float u = fminf(__fmul_rn(v, v), 32.0f);
-    float r = -1.0653262e-11f;
-    r = fmaf(r, u, 6.922505e-10f);
-    r = fmaf(r, u, -1.1965207e-08f);
-    r = fmaf(r, u, -1.775779e-07f);
-    r = fmaf(r, u, 1.01666847e-05f);
-    r = fmaf(r, u, -1.5548168e-04f);
-    r = fmaf(r, u, -1.0037289e-04f);
-    r = fmaf(r, u, 0.10483905f);
-    return fmaf(r, u, 2.3022087f);
+    float r = 4.3443146e-13f;
+    r = fmaf(r, u, -4.3081289e-11f);
+    r = fmaf(r, u, 1.6313341e-09f);
+    r = fmaf(r, u, -2.5466631e-08f);
+    r = fmaf(r, u, -7.5623149e-08f);
+    r = fmaf(r, u, 9.7798011e-06f);
+    r = fmaf(r, u, -1.5490042e-04f);
+    r = fmaf(r, u, -1.0019503e-04f);
+    r = fmaf(r, u, 0.10483802f);
+    return fmaf(r, u, 2.3022091f);
+}
+// The same three functions for float32 data, where the roundings of sum, reciprocal and product above would show: with e the
+// exponential of minus the argument's absolute value, v / (1 + e) is v - v e / (1 + e) for v > 0 and v e / (1 + e) below, so
+// that every rounding but the last is of something small.  v P(v) is then off by at most 2^-24 of itself, the fit, and 9 x
+// 2^-24 and the argument's rounding as parts of |v| P(-|v|), which is at most 0.17 (0.28 for SiLU).  Largest error on the CPU
+// restatement with exact exponentials, fine | short | v (1 + erf) / 2: GELU 1.0e-7 | 2.3e-7 | 1.6e-7 for v in 1 .. 2, 2.5e-7 |
+// 5.3e-7 | 4.5e-7 in 4 .. 6, 5.2e-8 | 4.7e-8 | 4.7e-8 in -2 .. -1, 2.6e-8 | 2.5e-8 | 4.8e-8 in -3 .. -2.
+// An infinity below gives NaN (the product of infinity and zero), as in the short forms; one above stays.
+__device__ __forceinline__ float fine_times(float v, float e) {
+    const float q = e * rcp_approx(1.0f + e), a = fmaxf(-v, fminf(v, 128.0f));        // |v|; e is 0 beyond 128
+    return fmaf(-a, q, max_nan(v, 0.0f));
+}
+// exp(-|u|): what the argument loses by its rounding is put back in first order.
+__device__ __forceinline__ float exp_fine(float u) {
+    const float a = fminf(fabsf(u), 128.0f), t = __fmul_rn(a, -1.44269504f), e = exp2_approx(t);
+    return fmaf(e, fmaf(t, -0.69314718f, -a), e);
 }
 // act(v) on N values at once: the choice is the same for the whole launch, so it is made once per N values.  A NaN stays
-// a NaN in every activation.
-template <int N>
+// a NaN in every activation.  kFine: for float32 data; 16-bit data round 2^13 times and more coarser than the short forms.
+template <bool kFine, int N>
 __device__ __forceinline__ void activate(int act, float (&v)[N]) {
     switch (act) {
         case kActRelu:
@@ -90,16 +105,25 @@ __device__ __forceinline__ void activate(int act, float (&v)[N]) {
             break;
         case kActSilu:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = logistic_times(v[i], v[i]);
+            for (int i = 0; i < N; ++i) {
+                if constexpr (kFine) v[i] = fine_times(v[i], exp_fine(v[i]));
+                else v[i] = logistic_times(v[i], v[i]);
+            }
             break;
         case kActGelu:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = v[i] * rcp_approx(1.0f + exp2_approx(-__fmul_rn(v[i], gelu_logit(v[i]))));
+            for (int i = 0; i < N; ++i) {
+                if constexpr (kFine) v[i] = fine_times(v[i], exp2_approx(-__fmul_rn(fabsf(v[i]), gelu_logit(v[i]))));
+                else v[i] = v[i] * rcp_approx(1.0f + exp2_approx(-__fmul_rn(v[i], gelu_logit(v[i]))));
+            }
             break;
         case kActGeluTanh:       // 0.5 v (1 + tanh u) = v / (1 + exp(-2u)), u = sqrt(2/pi) (v + 0.044715 v^3)
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                v[i] = logistic_times(v[i], 1.5957691f * fmaf(__fmul_rn(0.044715f * v[i], v[i]), v[i], v[i]));
+            for (int i = 0; i < N; ++i) {
+                const float u2 = 1.5957691f * fmaf(__fmul_rn(0.044715f * v[i], v[i]), v[i], v[i]);
+                if constexpr (kFine) v[i] = fine_times(v[i], exp_fine(u2));
+                else v[i] = logistic_times(v[i], u2);
+            }
             break;
         default: break;
     }
@@ -135,6 +159,8 @@ struct FusedEpilogue {
         if (bias_dtype == kDtypeBf16) return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[col]);
         return __half2float(static_cast<const __half*>(bias)[col]);
     }
+    template <int N>
+    __device__ __forceinline__ void activate(float (&v)[N]) const { tb200::activate<k32>(act, v); }
     // Before the activation.  Without a bias 0 is added, which only turns -0 into +0.
     __device__ __forceinline__ float linear(int32_t c, float rs, float cs, float b) const {
         return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(c), rs), cs), b);
@@ -159,7 +185,7 @@ struct FusedEpilogue {
     }
     __device__ __forceinline__ void store(int row, int col, int32_t c) const {
         float v[1] = {linear(c, row_scale[row], column_scale(col), column_bias(col))};
-        activate(act, v);
+        activate(v);
         finish(row, col, v[0]);
     }
 
@@ -279,7 +305,7 @@ struct FusedEpilogue {
         float v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = linear(c[i], rs, column_scale(col + i), column_bias(col + i));
-        activate(act, v);
+        activate(v);
         finish4(row, col, v, raw);
     }
 };

@@ -308,7 +308,7 @@ ternary_gemm_split_kernel(const __grid_constant__ CUtensorMap tmap_a, const __gr
 #pragma unroll
                 for (int x = 0; x < 4; ++x) v[4 * u + x] = epi.linear(sum[x], rs[u], cs[x], b[x]);
             }
-            activate(epi.act, v);
+            epi.activate(v);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
                 if (row[u] < M && col < N) epi.finish4(row[u], col, v + 4 * u, raw[u]);

@@ -605,7 +605,7 @@ ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid
                         v[j + 2] = epi.linear(static_cast<int32_t>(r[i][j + 2]) >> 6, __uint_as_float(rs.z), col_s, col_b);
                         v[j + 3] = epi.linear(static_cast<int32_t>(r[i][j + 3]) >> 6, __uint_as_float(rs.w), col_s, col_b);
                     }
-                    activate(epi.act, v);
+                    epi.activate(v);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) sts_u32(buf + ((j * 128 + colp) << 2), __float_as_uint(v[j]));
                     // Row by row from here: a warp has eight rows, a lane four columns.  The residual is requested before the

@@ -190,7 +190,7 @@ __device__ __forceinline__ void row_values(const RowQuantArgs& p, int row, int h
                                            const RowRaw<T, V> (&y)[VPT], float (&t)[VPT][V]) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) row_unpack<T, V>(x[j], t[j]);
-    if constexpr (MODE == kRowGate) activate(p.act, reinterpret_cast<float (&)[VPT * V]>(t));       // one choice for all of them
+    if constexpr (MODE == kRowGate) activate<std::is_same_v<T, float>>(p.act, reinterpret_cast<float (&)[VPT * V]>(t));       // one choice for all of them
     if constexpr (MODE != kRowNorm) {
         T* h = MODE == kRowNormResidual ? static_cast<T*>(p.h) + static_cast<long long>(row) * p.ldh + static_cast<int>(threadIdx.x * V) - shift : nullptr;
 #pragma unroll
@@ -515,7 +515,7 @@ __device__ __forceinline__ void row_single(const RowQuantArgs& p, int row, int k
         t[0] = to_float<T>(x.t[0]);
         x.store(static_cast<T*>(p.h) + static_cast<size_t>(row) * p.ldh + k);
     } else if constexpr (MODE == kRowGate) {
-        activate(p.act, t);
+        activate<std::is_same_v<T, float>>(p.act, t);
         t[0] = __fmul_rn(t[0], to_float<T>(y.t[0]));
     }
 }
