@@ -16,7 +16,7 @@
 // A row belongs to one CTA (a cluster, where rows are few and long), spread over its threads as VPT vectors of 16 bytes each.  Where rows start or end off a 16-byte
 // boundary the vectors are laid out so that their codes are aligned (the first and the last one may be partial), and a
 // vector of an input is put together from the two aligned pieces that it lies in: odd rows, and the halves of a product's
-// output with an odd width.
+// output with an odd width.  Two float32 inputs, and short rows of 16 bits, are taken as single elements there (launch_row_quant).
 //
 // Bound by memory: each input once, each output once.  Measured on B200 (copy rate 6.55 TB/s): gate 4096 x 28672 bfloat16 with
 // squared ReLU 91 us = 6.4 TB/s; with SiLU 112 us (two MUFU instructions an element, and an SM has room for one row, so its
@@ -342,22 +342,26 @@ __device__ __forceinline__ void row_finish(const RowQuantArgs& p, int row, int h
     for (int j = 0; j < VPT; ++j) {
         if (j >= have) continue;
         int8_t* at = q + j * blockDim.x * V;
-        uint32_t c[V / 4];
+        if constexpr (V == 1) {
+            *at = static_cast<int8_t>(row_code(t[j][0], r.inv) & r.keep);
+        } else {
+            uint32_t c[V / 4];
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i)
-            c[i] = pack_codes(row_code(t[j][4 * i], r.inv), row_code(t[j][4 * i + 1], r.inv),
-                              row_code(t[j][4 * i + 2], r.inv), row_code(t[j][4 * i + 3], r.inv)) & r.keep;
-        if constexpr (!kVec) {
-            const int k = static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift;
-            if (k < 0 || k + V > p.K) {
+            for (int i = 0; i < V / 4; ++i)
+                c[i] = pack_codes(row_code(t[j][4 * i], r.inv), row_code(t[j][4 * i + 1], r.inv),
+                                  row_code(t[j][4 * i + 2], r.inv), row_code(t[j][4 * i + 3], r.inv)) & r.keep;
+            if constexpr (!kVec) {
+                const int k = static_cast<int>((threadIdx.x + j * blockDim.x) * V) - shift;
+                if (k < 0 || k + V > p.K) {
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (k + i >= 0 && k + i < p.K) at[i] = static_cast<int8_t>(c[i / 4] >> (8 * (i & 3)));
-                continue;
+                    for (int i = 0; i < V; ++i)
+                        if (k + i >= 0 && k + i < p.K) at[i] = static_cast<int8_t>(c[i / 4] >> (8 * (i & 3)));
+                    continue;
+                }
             }
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(c[0], c[1]);
+            else *reinterpret_cast<uint32_t*>(at) = c[0];
         }
-        if constexpr (V == 8) *reinterpret_cast<uint2*>(at) = make_uint2(c[0], c[1]);
-        else *reinterpret_cast<uint32_t*>(at) = c[0];
     }
 }
 // Of `items` vectors those that fall to this thread: threadIdx.x, threadIdx.x + blockDim.x, ...
@@ -367,12 +371,13 @@ __device__ __forceinline__ int row_have(int items) {
 }
 
 // One row per CTA.  Of a row's operands and codes: all on vector boundaries; all equally far off one; anything else.
-constexpr int kRowAligned = 0, kRowSamePhase = 1, kRowAnyPhase = 2;
+// kRowElements takes the last kind too, a row as single elements instead of vectors.
+constexpr int kRowAligned = 0, kRowSamePhase = 1, kRowAnyPhase = 2, kRowElements = 3;
 template <typename T, int MODE, int VPT, int kForm>
 __global__ void __launch_bounds__(1024)
 row_quant_kernel(const __grid_constant__ RowQuantArgs p) {
-    constexpr int V = kRowVec<T>;
-    constexpr bool kVec = kForm == kRowAligned, kSame = kForm == kRowSamePhase;
+    constexpr int V = kForm == kRowElements ? 1 : kRowVec<T>;
+    constexpr bool kVec = kForm == kRowAligned || kForm == kRowElements, kSame = kForm == kRowSamePhase;
     __shared__ uint2 slots[2][32];
     const int row = blockIdx.x;
     int shift = 0;

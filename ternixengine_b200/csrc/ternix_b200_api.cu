@@ -1349,8 +1349,25 @@ int launch_row_quant(const tb200::RowQuantArgs& p, cudaStream_t st) {
             if (n <= 2048 && p.M <= sm_count()) return launch_row_quant_t<T, MODE, 2, kForm>(p, threads_for(n, 2), st);
             return launch_row_quant_t<T, MODE, 4, kForm>(p, threads_for(n, 4), st);
         };
-        if (items <= 4096)
-            return same ? launch(std::integral_constant<int, tb200::kRowSamePhase>{}) : launch(std::integral_constant<int, tb200::kRowAnyPhase>{});
+        // Single elements where putting vectors together costs more than their wider accesses save: two float32 inputs (three
+        // aligned pieces per vector for four elements, and spills at four vectors a thread; gate 512 x 8191 SiLU with the norm
+        // 26.2 | 13.1 us, 2048 x 4099 33.3 | 25, norm with residual 4096 x 8191 168 | 100; eight a thread as long as a CTA has an SM
+        // to itself, 1 x 4099 3.6, sixteen 4.4), and short rows of 16 bits, where a vector a thread leaves few threads (norm with
+        // residual 33 x 515 2.6 | 2.0 us, gate 1024 x 1001 4.2 | 4.1, but 4096 x 1001 10.0 | 12.9).
+        if (!same) {
+            if constexpr (sizeof(T) == 4 && MODE != tb200::kRowNorm) {
+                if (p.K <= 4096) return launch_row_quant_t<T, MODE, 4, tb200::kRowElements>(p, threads_for(p.K, 4), st);
+                if (p.K <= 8192 && p.M <= sm_count()) return launch_row_quant_t<T, MODE, 8, tb200::kRowElements>(p, threads_for(p.K, 8), st);
+                if (p.K <= 16384) return launch_row_quant_t<T, MODE, 16, tb200::kRowElements>(p, threads_for(p.K, 16), st);
+            } else if constexpr (sizeof(T) == 2) {
+                if (p.K <= 640 || (p.K <= 1024 && p.M <= 8 * sm_count()))
+                    return launch_row_quant_t<T, MODE, 4, tb200::kRowElements>(p, threads_for(p.K, 4), st);
+            }
+        }
+        if (items <= 4096) {
+            if (same) return launch(std::integral_constant<int, tb200::kRowSamePhase>{});
+            if constexpr (sizeof(T) == 2 || MODE == tb200::kRowNorm) return launch(std::integral_constant<int, tb200::kRowAnyPhase>{});
+        }
     }
     return launch_layer(tb200::row_quant_long_kernel<T, MODE>, dim3(static_cast<unsigned>(p.M)), 1024, 0, 1, st, p);
 }
