@@ -513,7 +513,8 @@ def rmsnorm_quantize(x, weight=None, residual=None, eps: float = 1e-5, out=None,
     x, residual: CUDA (M, K) bfloat16, float16 or float32, unit column stride, any row pitch.  weight: (K,) of the same
     type or float32, or None.  Returns (codes, row_scale), and h as a third where a residual is given; residual_out may be
     `residual` or `x` itself.  codes x row_scale stands for y: codes = rint(h * weight * 127 / max|h * weight|).  A row of
-    zeros has codes 0 and scale 1, a row with an infinity or NaN has codes 0 and scale NaN."""
+    zeros has codes 0 and scale 1, a row with an infinity or NaN has codes 0 and scale NaN.  No gradient is recorded: operands
+    that require one are read as they are, and the results require none."""
     rt = _runtime or _rt()
     if out is not None and row_scale is not None and rt.norm(x, weight, residual, eps, out, row_scale, residual_out) == 0:
         return (out, row_scale) if residual is None else (out, row_scale, residual_out)
@@ -554,8 +555,8 @@ def glu_quantize(gate, up, activation: str = "silu", weight=None, eps=None, out=
 
     gate, up: CUDA (M, K) of one type (bfloat16, float16 or float32), unit column stride, any row pitch, e.g. the two halves
     of one product's output.  activation: "none", "relu", "relu2", "silu", "gelu" or "gelu_tanh".  weight: (K,) of the same
-    type or float32, only with eps.  Returns (codes, row_scale); rows of zeros and rows with an infinity or NaN as in
-    rmsnorm_quantize()."""
+    type or float32, only with eps.  Returns (codes, row_scale); rows of zeros and rows with an infinity or NaN, and no
+    gradients, as in rmsnorm_quantize()."""
     rt = _runtime or _rt()
     act = ACTIVATIONS.get(activation)
     if out is not None and row_scale is not None and rt.glu(gate, up, act, weight, eps, out, row_scale) == 0:
@@ -596,7 +597,8 @@ def matmul_fused(a, w_packed, row_scale, w_scale=1.0, bias=None, activation: str
     w_scale: a number, or an (N,) float32 tensor.  bias: (N,) float32, bfloat16 or float16.  activation: "none", "relu",
     "relu2", "silu", "gelu" or "gelu_tanh".  residual: (M, N) of the output's type, unit column stride, any row pitch; may be
     `out` itself.  out: (M, N) bfloat16, float16 or float32, unit column stride, any row pitch; without it a new tensor of
-    out_dtype (the residual's type, else bfloat16).  status: an int32 on the same device, raised when a wait ran out."""
+    out_dtype (the residual's type, else bfloat16).  status: an int32 on the same device, raised when a wait ran out.  No
+    gradient is recorded, as in rmsnorm_quantize()."""
     rt = _runtime or _rt()
     act, kern = ACTIVATIONS.get(activation), KERNELS.get(kernel)
     if out is not None and status is None and out_dtype is None and \
