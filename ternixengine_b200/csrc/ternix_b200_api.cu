@@ -34,8 +34,11 @@ namespace {
 thread_local int g_last_cuda_error = 0;
 thread_local int g_last_launched = 0;      // TERNIX_B200_LAUNCHED_* of the calling thread's last single-product launch
 
+// The runtime keeps a failed call's error until it is asked for, and a later launch that succeeds would be reported as failed by
+// it: it is taken here (one that has lost the context comes back by itself).
 int cuda_fail(cudaError_t e) {
     g_last_cuda_error = static_cast<int>(e);
+    cudaGetLastError();
     return TERNIX_B200_ERR_CUDA;
 }
 #define TB_CUDA(call)                                            \
