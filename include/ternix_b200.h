@@ -40,7 +40,8 @@ extern "C" {
 #define TERNIX_B200_KERNEL_GEMV     2  /* decode regime, M <= 16: TMA-streamed packed W, dp4a         */
 #define TERNIX_B200_KERNEL_GEMM_TC  3  /* prefill regime: TMA + tcgen05 kind::i8, int32 in TMEM       */
 #define TERNIX_B200_KERNEL_DECODE_MMA 4 /* batched decode (a few to a few dozen rows): TMA-streamed   */
-                                       /* packed W decoded in registers into mma.sync.m16n8k32       */
+                                       /* packed W decoded in registers into mma.sync.m16n8k32; up to */
+                                       /* 65536 rows                                                  */
 #define TERNIX_B200_KERNEL_SKINNY_TC 5 /* batched decode, 1..128 rows: TMA-streamed packed W decoded  */
                                        /* into tensor memory as the A operand of tcgen05 kind::i8     */
 

@@ -12,8 +12,8 @@
 //
 // Measured on B200 (launches in a graph, weights in L2): a cluster takes 5 to 8 us from its launch to its last store and
 // 0.3 us per k-block of its pairs up to 128 rows (two issuers; with one 0.5), 0.55 us at 256 rows.  256 x 6912 x 2560 onto a
-// residual 11.3 us, cut 3 (cut 2 12.1; persistent 23 us; floor by the measured tensor rate 2.7 us); 32 x 4096 x 11008 with bias and SiLU 11 us
-// (mma.sync 15 us); 64 x 2560 x 2560 6.5 us.  The 0.3 us are the tensor pipe:
+// residual 10.9 us, cut 3 (cut 2 12.0; persistent 23 us; 1.9 us at the rate of the instruction, below, on all SMs); 32 x 4096 x 11008 with bias and SiLU 11 us
+// (mma.sync 15 us); 64 x 2560 x 2560 6.8 us.  The 0.3 us are the tensor pipe:
 // a k-block of 128 rows is 8 MMAs of 256 x 128 x 32, at 8192 products a clock and SM 64 clocks each, 0.27 us in all, and MMAs
 // of 64 rows take as long (256 rows: 0.54 us; measured 0.55).  Four issuers, a deeper operand ring (6 slots) and more expander
 // warps accordingly change nothing; what is left is SMs without a tile and the way in and out.

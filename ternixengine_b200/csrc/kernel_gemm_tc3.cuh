@@ -281,8 +281,8 @@ __device__ __forceinline__ void sts_u16(uint32_t saddr, uint16_t v) {
 // writes them to the staging buffer as fp32; the group's four warps read that back row by row, four columns to a lane, for
 // coalesced loads of the residual (kRes: there is one) and stores of the output (256 bytes of bfloat16 per row and warp)
 // at any pitch, without a TMA view.  Eight warps per CTA hold the accumulator, so what they do is bound by latency, not by
-// issue slots.  4096 x 2560 x 6912 to bfloat16, where ten k-blocks cover 5.7 us of it per tile: no activation 49.5 us (the
-// int32 product 48.6), SiLU 58.6, residual 56; done row by row on four values at a time, as first built, 128 with SiLU.
+// issue slots.  4096 x 2560 x 6912 to bfloat16, where ten k-blocks cover 5.7 us of it per tile: no activation 49 us (the
+// int32 product 48.6), SiLU 53, GELU 69, residual 54; to float32 none 51, SiLU 65, GELU 80; done row by row on four values at a time, as first built, 128 with SiLU.
 template <bool kGrouped, bool kBf16 = false, int TA = kTc3TileA, typename Epi = StoreInt32, bool kRes = false>
 __global__ void __launch_bounds__(kTc3Threads, 1)
 ternary_gemm_tc3_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,

@@ -19,10 +19,10 @@
 // output with an odd width.  Two float32 inputs, and short rows of 16 bits, are taken as single elements there (launch_row_quant).
 //
 // Bound by memory: each input once, each output once.  Measured on B200 (copy rate 6.55 TB/s): gate 4096 x 28672 bfloat16 with
-// squared ReLU 91 us = 6.4 TB/s; with SiLU 112 us (two MUFU instructions an element, and an SM has room for one row, so its
-// phases do not overlap); norm with residual 4096 x 8192 bfloat16 42 us = 5.6 TB/s, float32 70 us = 6.2 TB/s; 4096 x 2560
-// bfloat16 15.8 us.  One row: 1.9 us (2560), 2.2 us (6912 gate with the norm, a
-// cluster of eight), 2.4 us (28672), the launch and two trips through the reduction.
+// squared ReLU 91 us = 6.4 TB/s; with SiLU 115.5 us, GELU 127 (two MUFU instructions an element, and an SM has room for one row, so its
+// phases do not overlap); norm with residual 4096 x 8192 bfloat16 41.4 us = 5.7 TB/s, float32 70.5 us = 6.2 TB/s; 4096 x 2560
+// bfloat16 15.5 us.  One row: 1.8 us (2560), 2.2 us (6912 gate with the norm, a
+// cluster of eight), 2.3 us (28672), the launch and two trips through the reduction.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -1436,8 +1436,8 @@ struct SplitPlan {
 // Tile rows and cut with the smallest estimate, in microseconds as measured on B200 for 17 to 1500 rows, K 640 to 8192 and
 // N 640 to 28672: a cluster takes a fixed time (launch, first loads, the way out) and one per k-block of its pairs; clusters
 // beyond what the device holds at once come in waves.  The persistent form pays its way in and out once and afterwards the
-// longer of a tile's MMAs and a tile's epilogue.  E.g. 256 x 6912 x 2560: 11.3 us as 128 rows, cut 3, 12.1 us cut 2, 23.2 us persistent;
-// 1024 x 2560 x 6912: 32.5 us as 256 rows, uncut, 21.1 us persistent.
+// longer of a tile's MMAs and a tile's epilogue.  E.g. 256 x 6912 x 2560: 10.9 us as 128 rows, cut 3, 12.0 us cut 2, 23.0 us persistent;
+// 1024 x 2560 x 6912: 32.1 us as 256 rows, uncut, 20.8 us persistent.
 template <typename Epi>
 SplitPlan plan_split(int M, int K, int N) {
     const Options& o = options();
