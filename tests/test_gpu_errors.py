@@ -1,30 +1,43 @@
 """A call that failed is reported once: the calls after it are not blamed for it."""
-import numpy as np
+import os
+import subprocess
+import sys
+
 import pytest
 
-import oracle_lib
-import ternixengine_b200 as tb
-
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+# A group cannot be made while a stream captures (it allocates); the products after that are as good as ever.  In a process of its
+# own: a capture that was broken off leaves torch's random generator in capture mode.
+FAILS_ONCE = """
+import numpy as np, torch, oracle_lib, ternixengine_b200 as tb
+a, wp = tb.synth_activations((3, 33), 1), tb.synth_packed_weights(33, 36, 2)
+ta, tw = torch.from_numpy(a).cuda(), torch.from_numpy(wp).cuda()
+out = torch.empty(1, 64, dtype=torch.int32, device="cuda")
+ga, gw = torch.zeros(1, 64, dtype=torch.int8, device="cuda"), torch.zeros(64, 16, dtype=torch.uint8, device="cuda")
+rs, ones = torch.ones(3, device="cuda"), torch.ones(2, 64, device="cuda")
+torch.cuda.synchronize()
+failed = False
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            tb.ProjectionGroup([(ga, gw, out)])
+        except tb.TernixError:
+            failed = True
+except Exception:
+    pass                                  # the capture is void
+assert failed
+torch.cuda.synchronize()
+assert np.array_equal(tb.matmul(ta, tw, kernel="generic").cpu().numpy(), oracle_lib.matmul(a, wp))
+assert (tb.quantize_rows(ones)[0] == 127).all()
+y = tb.matmul_fused(ta, tw, rs, 1.0, out_dtype=torch.float32)
+assert np.array_equal(y.cpu().numpy(), oracle_lib.matmul(a, wp).astype(np.float32))
+print("as good as ever")
+"""
 
 
 def test_a_failed_call_does_not_fail_the_next_one():
-    """A group cannot be made while a stream captures (it allocates); the products after that are as good as ever."""
-    import torch
-    a, wp = tb.synth_activations((3, 33), 1), tb.synth_packed_weights(33, 36, 2)
-    ta, tw = torch.from_numpy(a).cuda(), torch.from_numpy(wp).cuda()
-    out = torch.empty(1, 64, dtype=torch.int32, device="cuda")
-    ga, gw = torch.zeros(1, 64, dtype=torch.int8, device="cuda"), torch.zeros(64, 16, dtype=torch.uint8, device="cuda")
-    torch.cuda.synchronize()
-    with pytest.raises(Exception):
-        with torch.cuda.graph(torch.cuda.CUDAGraph()):
-            with pytest.raises(tb.TernixError):
-                tb.ProjectionGroup([(ga, gw, out)])
-            raise RuntimeError("leave the capture")
-    torch.cuda.synchronize()
-    c = tb.matmul(ta, tw, kernel="generic")
-    assert np.array_equal(c.cpu().numpy(), oracle_lib.matmul(a, wp))
-    q, s = tb.quantize_rows(torch.ones(2, 64, device="cuda"))
-    assert (q == 127).all()
-    y = tb.matmul_fused(ta, tw, torch.ones(3, device="cuda"), 1.0, out_dtype=torch.float32)
-    assert np.array_equal(y.cpu().numpy(), oracle_lib.matmul(a, wp).astype(np.float32))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([ROOT, os.path.join(ROOT, "tests")]))
+    p = subprocess.run([sys.executable, "-c", FAILS_ONCE], capture_output=True, text=True, timeout=300, env=env)
+    assert p.returncode == 0 and "as good as ever" in p.stdout, p.stderr[-2000:]
